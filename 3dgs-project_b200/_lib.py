@@ -85,6 +85,13 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "gs3d_backward_preprocess_adam": (_I, [_P] * 6 + [_I, _P, _P, _SZ, _P, _SZ, _P, _P]),
     "adam_step_multi": (_I, [_I, _P, _I, ctypes.c_double, ctypes.c_double, ctypes.c_double, _P]),
     "adam_step_multi_lean": (_I, [_I, _P, _I, ctypes.c_double, ctypes.c_double, ctypes.c_double, _P, _LL, _P]),
+    "splat_grad_workspace_size": (_SZ, [_I]),
+    "splat_grad_norm": (_I, [_I, _P, _P, _P, _I, _P, _I, _P, _SZ, _P]),
+    "splat_grad_clip": (_I, [_I, _P, _P, _P, _P, _I, ctypes.c_double, _P, _I, _P, _SZ, _P]),
+    "adam_step_multi_clipped": (_I, [_I, _P, _I, ctypes.c_double, ctypes.c_double, ctypes.c_double, _I,
+                                     ctypes.c_double, _P, _P, _SZ, _P]),
+    "adam_step_multi_lean_clipped": (_I, [_I, _P, _I, ctypes.c_double, ctypes.c_double, ctypes.c_double, _P, _LL, _I,
+                                          ctypes.c_double, _P, _P, _SZ, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -12,6 +12,7 @@ import ctypes
 import torch
 
 from . import _lib as L
+from . import grad as gs_grad
 
 
 class _Group(ctypes.Structure):
@@ -51,11 +52,25 @@ class FusedAdam(torch.optim.Adam):
                           added inside the fused step). The parameters, moments and densification statistics are
                           bit-identical to the unfused path for one rendered view per step; with several views per
                           step all but the last are materialised into .grad when the next one arrives.
+      max_grad_norm       step() applies the gradients scaled by min(1, max_grad_norm / (norm + 1e-6)), norm the global
+                          norm of order grad_norm_type (1, 2 or inf) over every gradient of the step, which it leaves
+                          in `grad_norm` (0-d, on the device; no host read). .grad keeps the raw gradients; the
+                          update is that of grad.clip_grad_norm_ followed by the plain step, bit for bit. Not with
+                          fuse_backward, whose gradients are never written.
     """
 
     def __init__(self, params, lr, eps, betas=(0.9, 0.999), sparse: bool = False,
-                 lowp_moment_groups: tuple = (), fuse_backward: bool = False) -> None:
+                 lowp_moment_groups: tuple = (), fuse_backward: bool = False, max_grad_norm: float | None = None,
+                 grad_norm_type: float = 2.0) -> None:
+        if max_grad_norm is not None:
+            max_grad_norm = gs_grad.check_max_norm(max_grad_norm)
+            if fuse_backward:
+                raise RuntimeError("max_grad_norm needs the gradients that fuse_backward does not write")
+        gs_grad.norm_code(grad_norm_type)
         super().__init__(params=params, lr=lr, eps=eps, betas=betas)
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm_type = grad_norm_type
+        self.grad_norm: torch.Tensor | None = None  # of the last clipped step
         self.sparse = bool(sparse)
         self.lowp_moment_groups = set(lowp_moment_groups)
         self.lean = self.sparse or bool(self.lowp_moment_groups)
@@ -136,6 +151,8 @@ class FusedAdam(torch.optim.Adam):
     def step(self, closure=None) -> None:  # noqa: D102
         if closure is not None:
             raise RuntimeError("FusedAdam does not take a closure")
+        if self.max_grad_norm is not None:
+            self._check_clipped()
         done = self._fused_step() if self._pending is not None else set()
         visibility = None
         if self.sparse:
@@ -181,39 +198,104 @@ class FusedAdam(torch.optim.Adam):
                                    param.numel() // max(param.shape[0], 1), int(lowp))
             entry._keep = grad
             by_key.setdefault(key, []).append(entry)
+        clip = None
+        if self.max_grad_norm is not None:
+            clip = self._clip([e for groups in by_key.values() for e in groups],
+                              len(by_key) == 1 and max(map(len, by_key.values())) <= MAX_GROUPS)
         for key, groups in by_key.items():
             kind, step, b1, b2, eps, dev = key[:6]
-            stream = torch.cuda.current_stream(dev).cuda_stream
             for s in range(0, len(groups), MAX_GROUPS):
-                chunk = groups[s:s + MAX_GROUPS]
-                if kind == "dense":
-                    arr = (_Group * len(chunk))(*chunk)
-                    L.call("adam_step_multi", len(chunk), ctypes.addressof(arr), step, float(b1), float(b2),
-                           float(eps), stream)
-                else:
-                    vis = masks[key]
-                    arr = (_LeanGroup * len(chunk))(*chunk)
-                    L.call("adam_step_multi_lean", len(chunk), ctypes.addressof(arr), step, float(b1), float(b2),
-                           float(eps), L.ptr(vis), 0 if vis is None else vis.numel(), stream)
+                _launch(kind == "lean", groups[s:s + MAX_GROUPS], step, (b1, b2), eps, masks.get(key), dev, clip)
+
+    def _check_clipped(self) -> None:
+        """The clipped step's gradients: one norm is taken over them, on one device."""
+        devices = set()
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None and p.numel():
+                    L.check_cuda("param", p, torch.float32)
+                    if p.grad.dtype != torch.float32 or not p.grad.is_cuda or p.grad.layout != torch.strided:
+                        raise RuntimeError("max_grad_norm needs dense float32 CUDA gradients")
+                    devices.add(p.device)
+        if len(devices) > 1:
+            raise RuntimeError("max_grad_norm needs the parameters on one device")
+
+    def _clip(self, entries: list, in_step: bool):
+        """The clip arguments of the step's launches. A step of one launch takes the norm itself (in_step); for several
+        it is taken over all of their gradients first."""
+        norm = gs_grad.norm_code(self.grad_norm_type)
+        grads = [e._keep for e in entries]
+        if not grads:
+            self.grad_norm = torch.zeros(())
+            return None
+        if in_step:
+            self.grad_norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+            return norm, self.max_grad_norm, self.grad_norm
+        self.grad_norm = gs_grad.grad_norm(grads, self.grad_norm_type)
+        return gs_grad.NORM_GIVEN, self.max_grad_norm, self.grad_norm
 
 
-def adam_step(groups: list[tuple], step: int, betas=(0.9, 0.999), eps: float = 1e-15) -> None:
-    """Functional form: groups = [(param, grad, exp_avg, exp_avg_sq, lr), ...] (CUDA float32, contiguous)."""
-    if not groups:
+def _launch(lean: bool, groups: list, step: int, betas, eps: float, visibility, device, clip) -> None:
+    """One launch over at most MAX_GROUPS entries; `clip` = (norm code, max_norm, the norm's tensor) or None."""
+    arr = ((_LeanGroup if lean else _Group) * len(groups))(*groups)
+    args = [len(groups), ctypes.addressof(arr), int(step), float(betas[0]), float(betas[1]), float(eps)]
+    if lean:
+        args += [L.ptr(visibility), 0 if visibility is None else visibility.numel()]
+    name = "adam_step_multi_lean" if lean else "adam_step_multi"
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if clip is None:
+        L.call(name, *args, stream)
         return
-    arr = (_Group * len(groups))(*[_Group(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr))
-                                   for p, g, m, v, lr in groups])
-    L.call("adam_step_multi", len(groups), ctypes.addressof(arr), int(step), float(betas[0]), float(betas[1]),
-           float(eps), L.stream_of(groups[0][0]))
+    norm_type, max_norm, norm = clip
+    ws = None if norm_type == gs_grad.NORM_GIVEN else gs_grad.norm_workspace(len(groups), device)
+    with gs_grad.on_device(norm.get_device()):
+        L.call(name + "_clipped", *args, norm_type, max_norm, norm.data_ptr(), L.ptr(ws),
+               0 if ws is None else ws.numel(), stream)
+
+
+def _clip_args(groups: list[tuple], max_grad_norm, norm_type):
+    """adam_step's clip arguments, checked (its buffers' other checks are the caller's, as in the plain step)."""
+    code, limit = gs_grad.norm_code(norm_type), gs_grad.check_max_norm(max_grad_norm)
+    for i, group in enumerate(groups):
+        for name, t in zip(("param", "grad"), group):
+            L.check_cuda(f"{name} of group {i}", t, torch.float32)
+        for name, t in zip(("grad", "exp_avg", "exp_avg_sq"), group[1:4]):
+            L.check_cuda(f"{name} of group {i}", t)
+            if t.numel() != group[0].numel() or t.device != groups[0][0].device:
+                raise RuntimeError(f"{name} of group {i} must have its parameter's size, on the first group's device")
+    params = [g[0].data_ptr() for g in groups if g[0].numel()]
+    if len(set(params)) != len(params):
+        raise RuntimeError("a parameter appears in two groups")
+    return code, limit, torch.empty((), dtype=torch.float32, device=groups[0][0].device)
+
+
+def adam_step(groups: list[tuple], step: int, betas=(0.9, 0.999), eps: float = 1e-15,
+              max_grad_norm: float | None = None, norm_type: float = 2.0) -> torch.Tensor | None:
+    """Functional form: groups = [(param, grad, exp_avg, exp_avg_sq, lr), ...] (CUDA float32, contiguous).
+
+    With max_grad_norm the step takes the gradients times min(1, max_grad_norm / (norm + 1e-6)), norm the global norm
+    of order norm_type (1, 2 or inf) over the groups' gradients, and returns the norm (0-d, on the device). The
+    gradients keep their values."""
+    if not groups:
+        return None if max_grad_norm is None else torch.zeros(())
+    clip = None if max_grad_norm is None else _clip_args(groups, max_grad_norm, norm_type)
+    if clip is not None and any([v.dtype != torch.float32 for _, _, m, v, _ in groups for v in (m, v)]):
+        raise RuntimeError("moments must be float32 (adam_step_lean takes bfloat16 ones)")
+    entries = [_Group(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr))
+               for p, g, m, v, lr in groups]
+    _launch(False, entries, step, betas, eps, None, groups[0][0].device, clip)
+    return None if clip is None else clip[2]
 
 
 def adam_step_lean(groups: list[tuple], step: int, visibility: torch.Tensor | None = None, betas=(0.9, 0.999),
-                   eps: float = 1e-15) -> None:
+                   eps: float = 1e-15, max_grad_norm: float | None = None,
+                   norm_type: float = 2.0) -> torch.Tensor | None:
     """Functional lean form (the reference's `_C.adam_step_sparse` for several groups at once): groups =
     [(param, grad, exp_avg, exp_avg_sq, lr), ...]; exp_avg / exp_avg_sq float32 or bfloat16 (stochastic rounding);
-    visibility int32 [n_primitives] on the GPU or None."""
+    visibility int32 [n_primitives] on the GPU or None. max_grad_norm and norm_type as in adam_step; the norm counts the
+    gradients of primitives that are not visible too."""
     if not groups:
-        return
+        return None if max_grad_norm is None else torch.zeros(())
     entries = []
     for p, g, m, v, lr in groups:
         if m.dtype != v.dtype or m.dtype not in (torch.float32, torch.bfloat16):
@@ -222,6 +304,6 @@ def adam_step_lean(groups: list[tuple], step: int, visibility: torch.Tensor | No
             raise RuntimeError("visibility must be int32 [n_primitives] on CUDA")
         entries.append(_LeanGroup(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
                                   p.numel() // max(p.shape[0], 1), int(m.dtype == torch.bfloat16)))
-    arr = (_LeanGroup * len(entries))(*entries)
-    L.call("adam_step_multi_lean", len(entries), ctypes.addressof(arr), int(step), float(betas[0]), float(betas[1]),
-           float(eps), L.ptr(visibility), 0 if visibility is None else visibility.numel(), L.stream_of(groups[0][0]))
+    clip = None if max_grad_norm is None else _clip_args(groups, max_grad_norm, norm_type)
+    _launch(True, entries, step, betas, eps, visibility, groups[0][0].device, clip)
+    return None if clip is None else clip[2]

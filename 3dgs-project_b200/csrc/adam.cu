@@ -9,8 +9,11 @@
 // the group's buffers allow, so a step reads 4 and writes 3 floats per element and nothing else.
 // k_adam_lean adds the two options of the reference's lean Adam (adam_step_sparse_cu<LOWP>, same patch):
 // a per-primitive visibility mask and bfloat16 moments written with stochastic rounding.
+// Both kernels have a clipped form that multiplies each gradient by the clip factor of the global gradient norm
+// (grad_norm.cuh) as it is read, so that clipping costs the norm's read of the gradients and nothing else.
 #include "adam_math.cuh"
 #include "common.cuh"
+#include "grad_norm.cuh"
 
 namespace splat {
 namespace adam {
@@ -37,12 +40,21 @@ struct Table {
     float beta1, beta2, eps;
 };
 
-__device__ __forceinline__ float upd(float& p, float g, float& m, float& v, const Group& G, const Table& t) {
-    adam_element(p, g, m, v, G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
-    return p;
+// The gradient as the clipped step sees it: one product, rounded as the scaling kernel rounds it.
+template <bool kClip>
+__device__ __forceinline__ float clipped(float g, float factor) {
+    return kClip ? __fmul_rn(g, factor) : g;
 }
 
-__global__ void __launch_bounds__(kThreads) k_adam(Table t) {
+template <bool kClip>
+__device__ __forceinline__ void upd(float& p, float g, float& m, float& v, const Group& G, const Table& t,
+                                    float factor) {
+    adam_element(p, clipped<kClip>(g, factor), m, v, G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
+}
+
+template <bool kClip>
+__global__ void __launch_bounds__(kThreads) k_adam(Table t, gradnorm::Clip c) {
+    const float f = kClip ? static_cast<float>(gradnorm::block_factor(c, true)) : 1.f;
     int gi = 0;
 #pragma unroll 1
     while (gi + 1 < t.count && static_cast<long long>(blockIdx.x) >= t.g[gi + 1].first_block) ++gi;
@@ -57,20 +69,21 @@ __global__ void __launch_bounds__(kThreads) k_adam(Table t) {
                 const float4 g = __ldg(reinterpret_cast<const float4*>(G.grad + e));
                 float4 m = *reinterpret_cast<const float4*>(G.exp_avg + e);
                 float4 v = *reinterpret_cast<const float4*>(G.exp_avg_sq + e);
-                upd(p.x, g.x, m.x, v.x, G, t);
-                upd(p.y, g.y, m.y, v.y, G, t);
-                upd(p.z, g.z, m.z, v.z, G, t);
-                upd(p.w, g.w, m.w, v.w, G, t);
+                upd<kClip>(p.x, g.x, m.x, v.x, G, t, f);
+                upd<kClip>(p.y, g.y, m.y, v.y, G, t, f);
+                upd<kClip>(p.z, g.z, m.z, v.z, G, t, f);
+                upd<kClip>(p.w, g.w, m.w, v.w, G, t, f);
                 *reinterpret_cast<float4*>(G.param + e) = p;
                 *reinterpret_cast<float4*>(G.exp_avg + e) = m;
                 *reinterpret_cast<float4*>(G.exp_avg_sq + e) = v;
             } else {
-                for (long long j = e; j < G.n; ++j) upd(G.param[j], G.grad[j], G.exp_avg[j], G.exp_avg_sq[j], G, t);
+                for (long long j = e; j < G.n; ++j)
+                    upd<kClip>(G.param[j], G.grad[j], G.exp_avg[j], G.exp_avg_sq[j], G, t, f);
             }
         }
     } else {
         for (long long e = base + threadIdx.x; e < base + kPerBlock && e < G.n; e += kThreads)
-            upd(G.param[e], G.grad[e], G.exp_avg[e], G.exp_avg_sq[e], G, t);
+            upd<kClip>(G.param[e], G.grad[e], G.exp_avg[e], G.exp_avg_sq[e], G, t, f);
     }
 }
 
@@ -122,10 +135,10 @@ __device__ __forceinline__ long long primitive_of(const LeanGroup& G, long long 
     return i / G.features;
 }
 
-template <bool kLowp>
-__device__ __forceinline__ void lean_one(const LeanGroup& G, const LeanTable& t, long long i) {
+template <bool kLowp, bool kClip>
+__device__ __forceinline__ void lean_one(const LeanGroup& G, const LeanTable& t, long long i, float f) {
     if (t.visibility && t.visibility[primitive_of(G, i)] == 0) return;
-    const float g = G.grad[i];
+    const float g = clipped<kClip>(G.grad[i], f);
     float m, v;
     if (kLowp) {
         m = bf16_to_float(static_cast<const uint16_t*>(G.exp_avg)[i]);
@@ -169,8 +182,9 @@ __device__ __forceinline__ unsigned lean_mask(const LeanGroup& G, const LeanTabl
 
 // Four consecutive elements with vector accesses, `mask` from lean_mask (non-zero): elements of primitives that
 // are not visible keep their parameter and moments.
-template <bool kLowp>
-__device__ __forceinline__ void lean_four(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask) {
+template <bool kLowp, bool kClip>
+__device__ __forceinline__ void lean_four(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask,
+                                          float f) {
     bool on[kVec];
 #pragma unroll
     for (int k = 0; k < kVec; ++k) on[k] = (mask >> k) & 1u;
@@ -197,7 +211,7 @@ __device__ __forceinline__ void lean_four(const LeanGroup& G, const LeanTable& t
 #pragma unroll
     for (int k = 0; k < kVec; ++k) {
         if (!on[k]) continue;
-        adam_element(pv[k], gv[k], mv[k], vv[k], G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
+        adam_element(pv[k], clipped<kClip>(gv[k], f), mv[k], vv[k], G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
         const float m = mv[k], v = vv[k];
         if (kLowp) {
             const uint32_t r1 = lowbias32(static_cast<uint32_t>(e + k) ^ t.seed);
@@ -217,8 +231,8 @@ __device__ __forceinline__ void lean_four(const LeanGroup& G, const LeanTable& t
     }
 }
 
-template <bool kLowp>
-__device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base) {
+template <bool kLowp, bool kClip>
+__device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, float f) {
     if (G.vec) {
         // the visibility of all of this thread's groups of four first, so that their loads overlap one another
         // instead of each one delaying its group's data loads
@@ -233,27 +247,29 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
         for (int k = 0; k < kIters; ++k) {
             const long long e = base + (static_cast<long long>(k) * kThreads + threadIdx.x) * kVec;
             if (e + kVec <= G.n) {
-                if (mask[k]) lean_four<kLowp>(G, t, e, mask[k]);
+                if (mask[k]) lean_four<kLowp, kClip>(G, t, e, mask[k], f);
             } else {
-                for (long long j = e; j < G.n; ++j) lean_one<kLowp>(G, t, j);
+                for (long long j = e; j < G.n; ++j) lean_one<kLowp, kClip>(G, t, j, f);
             }
         }
     } else {
         for (long long e = base + threadIdx.x; e < base + kPerBlock && e < G.n; e += kThreads)
-            lean_one<kLowp>(G, t, e);
+            lean_one<kLowp, kClip>(G, t, e, f);
     }
 }
 
-__global__ void __launch_bounds__(kThreads) k_adam_lean(LeanTable t) {
+template <bool kClip>
+__global__ void __launch_bounds__(kThreads) k_adam_lean(LeanTable t, gradnorm::Clip c) {
+    const float f = kClip ? static_cast<float>(gradnorm::block_factor(c, true)) : 1.f;
     int gi = 0;
 #pragma unroll 1
     while (gi + 1 < t.count && static_cast<long long>(blockIdx.x) >= t.g[gi + 1].first_block) ++gi;
     const LeanGroup& G = t.g[gi];
     const long long base = (static_cast<long long>(blockIdx.x) - G.first_block) * kPerBlock;
     if (G.lowp)
-        lean_block<true>(G, t, base);
+        lean_block<true, kClip>(G, t, base, f);
     else
-        lean_block<false>(G, t, base);
+        lean_block<false, kClip>(G, t, base, f);
 }
 
 }  // namespace adam
@@ -268,16 +284,12 @@ void bias_corrections(double lr, double beta1, double beta2, int step, float& st
     adam_bias_corrections(lr, beta1, beta2, step, step_size, bc2_sqrt_rcp);
 }
 
-}  // namespace
-
-extern "C" {
-
-int adam_step_multi(int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
-                    void* stream) {
-    SPLAT_REQUIRE(count >= 0 && count <= SPLAT_ADAM_MAX_GROUPS, "adam_step_multi: %d groups (at most %d)", count,
+// The kernel's table for `count` groups; *blocks is 0 when every group is empty.
+int build_table(const char* what, int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
+                adam::Table& t, long long* total_blocks) {
+    SPLAT_REQUIRE(count >= 0 && count <= SPLAT_ADAM_MAX_GROUPS, "%s: %d groups (at most %d)", what, count,
                   SPLAT_ADAM_MAX_GROUPS);
-    SPLAT_REQUIRE(step >= 1, "adam_step_multi: step must be >= 1");
-    adam::Table t{};
+    SPLAT_REQUIRE(step >= 1, "%s: step must be >= 1", what);
     t.beta1 = static_cast<float>(beta1);
     t.beta2 = static_cast<float>(beta2);
     t.eps = static_cast<float>(eps);
@@ -285,9 +297,9 @@ int adam_step_multi(int count, const adam_group* groups, int step, double beta1,
     int k = 0;
     for (int i = 0; i < count; ++i) {
         const adam_group& g = groups[i];
-        SPLAT_REQUIRE(g.n >= 0, "adam_step_multi: group %d has negative size", i);
+        SPLAT_REQUIRE(g.n >= 0, "%s: group %d has negative size", what, i);
         if (g.n == 0) continue;
-        SPLAT_REQUIRE(g.param && g.grad && g.exp_avg && g.exp_avg_sq, "adam_step_multi: group %d has a null buffer", i);
+        SPLAT_REQUIRE(g.param && g.grad && g.exp_avg && g.exp_avg_sq, "%s: group %d has a null buffer", what, i);
         adam::Group& G = t.g[k++];
         G.param = g.param;
         G.grad = g.grad;
@@ -301,20 +313,17 @@ int adam_step_multi(int count, const adam_group* groups, int step, double beta1,
         blocks += (g.n + adam::kPerBlock - 1) / adam::kPerBlock;
     }
     t.count = k;
-    if (blocks == 0) return SPLAT_OK;
-    SPLAT_REQUIRE(blocks < (1ll << 31), "adam_step_multi: too many elements");
-    SPLAT_TIMED_LAUNCH("k_adam", as_stream(stream),
-                       (adam::k_adam<<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(t)));
-    note_launch();
-    return check_launch("adam_step_multi");
+    SPLAT_REQUIRE(blocks < (1ll << 31), "%s: too many elements", what);
+    *total_blocks = blocks;
+    return SPLAT_OK;
 }
 
-int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, double beta1, double beta2,
-                         double eps, const int32_t* visibility, long long n_primitives, void* stream) {
-    SPLAT_REQUIRE(count >= 0 && count <= SPLAT_ADAM_MAX_GROUPS, "adam_step_multi_lean: %d groups (at most %d)",
-                  count, SPLAT_ADAM_MAX_GROUPS);
-    SPLAT_REQUIRE(step >= 1, "adam_step_multi_lean: step must be >= 1");
-    adam::LeanTable t{};
+int build_lean_table(const char* what, int count, const adam_lean_group* groups, int step, double beta1, double beta2,
+                     double eps, const int32_t* visibility, long long n_primitives, adam::LeanTable& t,
+                     long long* total_blocks) {
+    SPLAT_REQUIRE(count >= 0 && count <= SPLAT_ADAM_MAX_GROUPS, "%s: %d groups (at most %d)", what, count,
+                  SPLAT_ADAM_MAX_GROUPS);
+    SPLAT_REQUIRE(step >= 1, "%s: step must be >= 1", what);
     t.beta1 = static_cast<float>(beta1);
     t.beta2 = static_cast<float>(beta2);
     t.eps = static_cast<float>(eps);
@@ -324,12 +333,11 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
     int k = 0;
     for (int i = 0; i < count; ++i) {
         const adam_lean_group& g = groups[i];
-        SPLAT_REQUIRE(g.n >= 0 && g.features >= 1, "adam_step_multi_lean: group %d has a bad size", i);
+        SPLAT_REQUIRE(g.n >= 0 && g.features >= 1, "%s: group %d has a bad size", what, i);
         if (g.n == 0) continue;
-        SPLAT_REQUIRE(g.param && g.grad && g.exp_avg && g.exp_avg_sq, "adam_step_multi_lean: group %d has a null buffer",
-                      i);
+        SPLAT_REQUIRE(g.param && g.grad && g.exp_avg && g.exp_avg_sq, "%s: group %d has a null buffer", what, i);
         SPLAT_REQUIRE(!visibility || g.n == static_cast<long long>(g.features) * n_primitives,
-                      "adam_step_multi_lean: group %d has %lld elements, not %d x %lld primitives", i, g.n, g.features,
+                      "%s: group %d has %lld elements, not %d x %lld primitives", what, i, g.n, g.features,
                       n_primitives);
         adam::LeanGroup& G = t.g[k++];
         G.param = g.param;
@@ -347,11 +355,101 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
         blocks += (g.n + adam::kPerBlock - 1) / adam::kPerBlock;
     }
     t.count = k;
+    SPLAT_REQUIRE(blocks < (1ll << 31), "%s: too many elements", what);
+    *total_blocks = blocks;
+    return SPLAT_OK;
+}
+
+// The clip factor's source for the groups' gradients: the caller's norm, or partials enqueued here.
+template <typename G>
+int clip_of(const char* what, int count, const G* groups, int norm_type, double max_norm, float* norm, void* workspace,
+            size_t workspace_bytes, cudaStream_t st, gradnorm::Clip& c) {
+    const bool given = norm_type == SPLAT_NORM_GIVEN;
+    SPLAT_REQUIRE(given || gradnorm::known_norm(norm_type), "%s: unknown norm type %d", what, norm_type);
+    SPLAT_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", what);
+    SPLAT_REQUIRE(norm, "%s: the norm's buffer is missing", what);
+    SPLAT_REQUIRE(given || (workspace && workspace_bytes >= splat_grad_workspace_size(count)),
+                  "%s: workspace too small", what);
+    c = {static_cast<const double*>(workspace), 0, norm_type, given, 0, norm, max_norm};
+    if (given) return SPLAT_OK;
+    const void* grads[SPLAT_ADAM_MAX_GROUPS];
+    long long n[SPLAT_ADAM_MAX_GROUPS];
+    unsigned char dtypes[SPLAT_ADAM_MAX_GROUPS] = {};  // SPLAT_F32
+    for (int i = 0; i < count; ++i) {
+        grads[i] = groups[i].grad;
+        n[i] = groups[i].n;
+    }
+    return gradnorm::enqueue_partials(count, grads, n, dtypes, norm_type, static_cast<double*>(workspace), &c.count, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int adam_step_multi(int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
+                    void* stream) {
+    adam::Table t{};
+    long long blocks = 0;
+    SPLAT_TRY(build_table("adam_step_multi", count, groups, step, beta1, beta2, eps, t, &blocks));
     if (blocks == 0) return SPLAT_OK;
-    SPLAT_REQUIRE(blocks < (1ll << 31), "adam_step_multi_lean: too many elements");
-    adam::k_adam_lean<<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(t);
+    SPLAT_TIMED_LAUNCH("k_adam", as_stream(stream),
+                       (adam::k_adam<false><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(
+                           t, gradnorm::Clip{})));
+    note_launch();
+    return check_launch("adam_step_multi");
+}
+
+int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, double beta1, double beta2,
+                         double eps, const int32_t* visibility, long long n_primitives, void* stream) {
+    adam::LeanTable t{};
+    long long blocks = 0;
+    SPLAT_TRY(build_lean_table("adam_step_multi_lean", count, groups, step, beta1, beta2, eps, visibility, n_primitives,
+                               t, &blocks));
+    if (blocks == 0) return SPLAT_OK;
+    adam::k_adam_lean<false><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(
+        t, gradnorm::Clip{});
     note_launch();
     return check_launch("adam_step_multi_lean");
+}
+
+int adam_step_multi_clipped(int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
+                            int norm_type, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    adam::Table t{};
+    long long blocks = 0;
+    SPLAT_TRY(build_table("adam_step_multi_clipped", count, groups, step, beta1, beta2, eps, t, &blocks));
+    const cudaStream_t st = as_stream(stream);
+    gradnorm::Clip c;
+    SPLAT_TRY(clip_of("adam_step_multi_clipped", count, groups, norm_type, max_norm, norm, workspace, workspace_bytes,
+                      st, c));
+    if (blocks == 0)  // the norm of nothing is the call's all the same
+        return c.given ? SPLAT_OK
+                       : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,
+                                         stream);
+    SPLAT_TIMED_LAUNCH("k_adam", st,
+                       (adam::k_adam<true><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, st>>>(t, c)));
+    note_launch();
+    return check_launch("adam_step_multi_clipped");
+}
+
+int adam_step_multi_lean_clipped(int count, const adam_lean_group* groups, int step, double beta1, double beta2,
+                                 double eps, const int32_t* visibility, long long n_primitives, int norm_type,
+                                 double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    adam::LeanTable t{};
+    long long blocks = 0;
+    SPLAT_TRY(build_lean_table("adam_step_multi_lean_clipped", count, groups, step, beta1, beta2, eps, visibility,
+                               n_primitives, t, &blocks));
+    const cudaStream_t st = as_stream(stream);
+    gradnorm::Clip c;
+    SPLAT_TRY(clip_of("adam_step_multi_lean_clipped", count, groups, norm_type, max_norm, norm, workspace,
+                      workspace_bytes, st, c));
+    if (blocks == 0)
+        return c.given ? SPLAT_OK
+                       : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,
+                                         stream);
+    adam::k_adam_lean<true><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, st>>>(t, c);
+    note_launch();
+    return check_launch("adam_step_multi_lean_clipped");
 }
 
 }  // extern "C"

@@ -384,6 +384,45 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
                          double eps, const int32_t* visibility, long long n_primitives, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Global gradient norm, clipping by it, and the Adam steps that clip (no counterpart in the reference).
+ *   norm = (sum |g|^p)^(1/p) over every element of every tensor, p = 1 or 2, or max |g|; sums in float64, in an order
+ *          fixed by the sizes (the same call gives the same bits); NaN when an element is NaN
+ *   f = min(1, max_norm / (norm + 1e-6)), NaN when the norm is; computed in float64 from the rounded norm
+ * A list of `count` tensors is given as host arrays: device pointers (aligned to their type, no other alignment
+ * needed), element counts, and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements may have null pointers.
+ * The arrays are read during the call only. *norm is device memory: float32, or float64 when norm_is_f64, which a list
+ * with a float64 tensor needs.
+ * workspace: device scratch of splat_grad_workspace_size(count) bytes, not kept between calls; calls that may run at
+ * the same time (other streams, graphs replayed side by side) need one each.
+ * ------------------------------------------------------------------------------------------- */
+#define SPLAT_F32 0
+#define SPLAT_BF16 1
+#define SPLAT_F16 2
+#define SPLAT_F64 3
+#define SPLAT_NORM_INF 0
+#define SPLAT_NORM_L1 1
+#define SPLAT_NORM_L2 2
+#define SPLAT_NORM_GIVEN 3 /* clipping calls: *norm is the caller's and is read instead of computed */
+size_t splat_grad_workspace_size(int count);
+int splat_grad_norm(int count, const void* const* grads, const long long* n, const unsigned char* dtypes, int norm_type,
+                    void* norm, int norm_is_f64, void* workspace, size_t workspace_bytes, void* stream);
+/* outs[i] = grads[i] * f, rounded once to the tensor's type (the product of a 16-bit tensor is taken in float32, that
+ * of a float32 one by f rounded to float32). outs[i] == grads[i] for every tensor clips in place (where f = 1 nothing
+ * is written), otherwise no output may overlap an input; outputs never overlap one another. */
+int splat_grad_clip(int count, const void* const* grads, void* const* outs, const long long* n,
+                    const unsigned char* dtypes, int norm_type, double max_norm, void* norm, int norm_is_f64,
+                    void* workspace, size_t workspace_bytes, void* stream);
+/* adam_step_multi / adam_step_multi_lean of the gradients grad * f, f from the norm over the groups of this call (with
+ * SPLAT_NORM_GIVEN: from *norm). The gradients are left as they are. Bit-identical to splat_grad_clip followed by the
+ * step. The norm counts every gradient, those of primitives that the lean step's mask leaves out too. */
+int adam_step_multi_clipped(int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
+                            int norm_type, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                            void* stream);
+int adam_step_multi_lean_clipped(int count, const adam_lean_group* groups, int step, double beta1, double beta2,
+                                 double eps, const int32_t* visibility, long long n_primitives, int norm_type,
+                                 double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Data-parallel Adam over peer memory (multi-view training on one node; the reference has no multi-GPU
  * path, so none of these has a counterpart in it). Buffers that other GPUs address directly: allocated
  * with splat_peer_alloc (zeroed; ipc_handle receives 64 bytes to send to the other ranks), mapped on
