@@ -8,6 +8,7 @@ round-trips with torch's Adam and with checkpoints written by the reference's tr
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -160,6 +161,7 @@ class FusedAdam(torch.optim.Adam):
 
             visibility = gs3d._Rasterize.last_visibility
         by_key: dict[tuple, list] = {}
+        grads: list[torch.Tensor] = []  # in the parameters' order, which the clip's sums follow
         masks: dict[tuple, torch.Tensor | None] = {}
         for group in self.param_groups:
             if len(group["params"]) != 1:
@@ -197,11 +199,11 @@ class FusedAdam(torch.optim.Adam):
                                    state["exp_avg_sq"].data_ptr(), param.numel(), float(group["lr"]),
                                    param.numel() // max(param.shape[0], 1), int(lowp))
             entry._keep = grad
+            grads.append(grad)
             by_key.setdefault(key, []).append(entry)
         clip = None
         if self.max_grad_norm is not None:
-            clip = self._clip([e for groups in by_key.values() for e in groups],
-                              len(by_key) == 1 and max(map(len, by_key.values())) <= MAX_GROUPS)
+            clip = self._clip(grads, len(by_key) == 1 and len(grads) <= MAX_GROUPS)
         for key, groups in by_key.items():
             kind, step, b1, b2, eps, dev = key[:6]
             for s in range(0, len(groups), MAX_GROUPS):
@@ -220,11 +222,10 @@ class FusedAdam(torch.optim.Adam):
         if len(devices) > 1:
             raise RuntimeError("max_grad_norm needs the parameters on one device")
 
-    def _clip(self, entries: list, in_step: bool):
+    def _clip(self, grads: list, in_step: bool):
         """The clip arguments of the step's launches. A step of one launch takes the norm itself (in_step); for several
         it is taken over all of their gradients first."""
         norm = gs_grad.norm_code(self.grad_norm_type)
-        grads = [e._keep for e in entries]
         if not grads:
             self.grad_norm = torch.zeros(())
             return None
@@ -248,25 +249,60 @@ def _launch(lean: bool, groups: list, step: int, betas, eps: float, visibility, 
         return
     norm_type, max_norm, norm = clip
     ws = None if norm_type == gs_grad.NORM_GIVEN else gs_grad.norm_workspace(len(groups), device)
-    with gs_grad.on_device(norm.get_device()):
+    with torch.cuda.device(device):
         L.call(name + "_clipped", *args, norm_type, max_norm, norm.data_ptr(), L.ptr(ws),
                0 if ws is None else ws.numel(), stream)
 
 
-def _clip_args(groups: list[tuple], max_grad_norm, norm_type):
-    """adam_step's clip arguments, checked (its buffers' other checks are the caller's, as in the plain step)."""
-    code, limit = gs_grad.norm_code(norm_type), gs_grad.check_max_norm(max_grad_norm)
-    for i, group in enumerate(groups):
-        for name, t in zip(("param", "grad"), group):
-            L.check_cuda(f"{name} of group {i}", t, torch.float32)
-        for name, t in zip(("grad", "exp_avg", "exp_avg_sq"), group[1:4]):
-            L.check_cuda(f"{name} of group {i}", t)
-            if t.numel() != group[0].numel() or t.device != groups[0][0].device:
+def _refuse_groups(groups: list[tuple], lean: bool) -> None:
+    """Raises for the first buffer that a clipped step does not take."""
+    for i, (p, g, m, v, _) in enumerate(groups):
+        moments = (torch.float32, torch.bfloat16) if lean else (torch.float32,)
+        for name, t in (("param", p), ("grad", g), ("exp_avg", m), ("exp_avg_sq", v)):
+            L.check_cuda(f"{name} of group {i}", t, torch.float32 if name in ("param", "grad") else None)
+            if t.dtype not in moments or (t is v and t.dtype != m.dtype):
+                raise RuntimeError(f"moments of group {i} must be float32" + (", or both bfloat16" if lean else
+                                   " (adam_step_lean takes bfloat16 ones)"))
+            if t.numel() != p.numel() or t.device != groups[0][0].device:
                 raise RuntimeError(f"{name} of group {i} must have its parameter's size, on the first group's device")
-    params = [g[0].data_ptr() for g in groups if g[0].numel()]
-    if len(set(params)) != len(params):
+    raise RuntimeError("the groups cannot be read as dense CUDA tensors")
+
+
+def _clipped_step(groups: list[tuple], lean: bool, step: int, betas, eps: float, visibility, max_grad_norm,
+                  norm_type) -> torch.Tensor:
+    """adam_step / adam_step_lean with max_grad_norm: the buffers of all groups read and checked in one go."""
+    code, limit = gs_grad.norm_code(norm_type), gs_grad.check_max_norm(max_grad_norm)
+    count = len(groups)
+    params, grads, exp_avg, exp_avg_sq, lrs = zip(*groups)
+    d = gs_grad.describe([*params, *grads, *exp_avg, *exp_avg_sq])
+    if d is None:
+        _refuse_groups(groups, lean)
+    size, kinds = 8 * count, d.codes[2 * count:3 * count]
+    sizes = d.sizes[:size]
+    if not d.contiguous or any(d.codes[:2 * count]) or d.codes[3 * count:] != kinds \
+            or max(kinds) > int(lean) or d.sizes != sizes * 4:
+        _refuse_groups(groups, lean)
+    address = struct.unpack(f"{4 * count}Q", d.addresses)
+    n = struct.unpack(f"{count}q", sizes)
+    used = [a for a, k in zip(address, n) if k]
+    if len(set(used)) != len(used):
         raise RuntimeError("a parameter appears in two groups")
-    return code, limit, torch.empty((), dtype=torch.float32, device=groups[0][0].device)
+    rows = []
+    for k in range(count):
+        rows += address[k::count]
+        rows += (n[k], float(lrs[k]))
+        if lean:
+            rows += (n[k] // max(params[k].shape[0], 1), kinds[k])
+    table = struct.pack(("PPPPqdii" if lean else "PPPPqd") * count, *rows)
+    device = params[0].device
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    ws = gs_grad.norm_workspace(count, device)
+    args = [count, table, int(step), float(betas[0]), float(betas[1]), float(eps)]
+    if lean:
+        args += [L.ptr(visibility), 0 if visibility is None else visibility.numel()]
+    d.call("adam_step_multi_lean_clipped" if lean else "adam_step_multi_clipped", *args, code, limit, norm.data_ptr(),
+           ws.data_ptr(), ws.numel())
+    return norm
 
 
 def adam_step(groups: list[tuple], step: int, betas=(0.9, 0.999), eps: float = 1e-15,
@@ -278,13 +314,12 @@ def adam_step(groups: list[tuple], step: int, betas=(0.9, 0.999), eps: float = 1
     gradients keep their values."""
     if not groups:
         return None if max_grad_norm is None else torch.zeros(())
-    clip = None if max_grad_norm is None else _clip_args(groups, max_grad_norm, norm_type)
-    if clip is not None and any([v.dtype != torch.float32 for _, _, m, v, _ in groups for v in (m, v)]):
-        raise RuntimeError("moments must be float32 (adam_step_lean takes bfloat16 ones)")
+    if max_grad_norm is not None:
+        return _clipped_step(groups, False, step, betas, eps, None, max_grad_norm, norm_type)
     entries = [_Group(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr))
                for p, g, m, v, lr in groups]
-    _launch(False, entries, step, betas, eps, None, groups[0][0].device, clip)
-    return None if clip is None else clip[2]
+    _launch(False, entries, step, betas, eps, None, groups[0][0].device, None)
+    return None
 
 
 def adam_step_lean(groups: list[tuple], step: int, visibility: torch.Tensor | None = None, betas=(0.9, 0.999),
@@ -296,14 +331,19 @@ def adam_step_lean(groups: list[tuple], step: int, visibility: torch.Tensor | No
     gradients of primitives that are not visible too."""
     if not groups:
         return None if max_grad_norm is None else torch.zeros(())
+    if visibility is not None and (visibility.dtype != torch.int32 or not visibility.is_cuda):
+        raise RuntimeError("visibility must be int32 [n_primitives] on CUDA")
+    if max_grad_norm is not None:
+        if visibility is not None:
+            L.check_cuda("visibility", visibility)
+            if visibility.device != groups[0][0].device:
+                raise RuntimeError("visibility must be on the groups' device")
+        return _clipped_step(groups, True, step, betas, eps, visibility, max_grad_norm, norm_type)
     entries = []
     for p, g, m, v, lr in groups:
         if m.dtype != v.dtype or m.dtype not in (torch.float32, torch.bfloat16):
             raise RuntimeError("moments must share a dtype, float32 or bfloat16")
-        if visibility is not None and (visibility.dtype != torch.int32 or not visibility.is_cuda):
-            raise RuntimeError("visibility must be int32 [n_primitives] on CUDA")
         entries.append(_LeanGroup(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
                                   p.numel() // max(p.shape[0], 1), int(m.dtype == torch.bfloat16)))
-    clip = None if max_grad_norm is None else _clip_args(groups, max_grad_norm, norm_type)
-    _launch(True, entries, step, betas, eps, visibility, groups[0][0].device, clip)
-    return None if clip is None else clip[2]
+    _launch(True, entries, step, betas, eps, visibility, groups[0][0].device, None)
+    return None

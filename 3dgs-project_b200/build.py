@@ -1,8 +1,8 @@
-"""Builds libsplat_b200.so (all csrc/*.cu for sm_100a) in place with nvcc.
+"""Builds libsplat_b200.so (all csrc/*.cu for sm_100a, nvcc) and _tensors.so (csrc/tensor_list.cpp, g++) in place.
 
     python 3dgs-project_b200/build.py [--force] [--verbose]
 
-Objects go to csrc/_build/ (git-ignored); the shared library lands next to this file so it travels
+Objects go to csrc/_build/ (git-ignored); the shared libraries land next to this file so they travel
 with the source tree. A rebuild happens only when a source, header or flag changed.
 """
 from __future__ import annotations
@@ -10,10 +10,12 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,6 +24,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = CSRC / "_build"
 LIB = PKG / "libsplat_b200.so"
+TENSORS = PKG / "_tensors.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -44,7 +47,33 @@ def _digest(sources: list[Path]) -> str:
     return h.hexdigest()
 
 
+def build_tensors(force: bool = False, verbose: bool = False) -> Path:
+    """The host-only module that reads lists of torch tensors: g++ against this interpreter's and torch's headers."""
+    torch_dir = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+    src = CSRC / "tensor_list.cpp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", str(src), f"-I{torch_dir / 'include'}",
+           f"-I{torch_dir / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{Path(nvcc()).resolve().parent.parent / 'include'}", f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python"]
+    version = (torch_dir / "version.py").read_bytes()
+    digest = hashlib.sha256(src.read_bytes() + version + " ".join([sys.version, *cmd]).encode()).hexdigest()
+    stamp = BUILD / "stamp_tensors"
+    if not force and TENSORS.exists() and stamp.exists() and stamp.read_text() == digest:
+        return TENSORS
+    BUILD.mkdir(parents=True, exist_ok=True)
+    tmp = TENSORS.with_suffix(".so.tmp")
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run([*cmd, "-o", str(tmp)], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TENSORS)
+    stamp.write_text(digest)
+    return TENSORS
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_tensors(force, verbose)
     sources = sorted(CSRC.glob("*.cu"))
     stamp = BUILD / "stamp"
     digest = _digest(sources)

@@ -11,6 +11,8 @@
 // a per-primitive visibility mask and bfloat16 moments written with stochastic rounding.
 // Both kernels have a clipped form that multiplies each gradient by the clip factor of the global gradient norm
 // (grad_norm.cuh) as it is read, so that clipping costs the norm's read of the gradients and nothing else.
+#include <algorithm>
+
 #include "adam_math.cuh"
 #include "common.cuh"
 #include "grad_norm.cuh"
@@ -21,6 +23,9 @@ namespace adam {
 constexpr int kThreads = 256;
 constexpr int kVec = 4;
 constexpr int kPerBlock = kThreads * kVec * 4;  // 4096 elements per block
+static_assert(kThreads == gradnorm::kTeam, "the small kernels split a block into teams of one tile");
+
+using GradTable = gradnorm::Table<SPLAT_ADAM_MAX_GROUPS>;
 
 struct Group {
     float* param;
@@ -46,27 +51,30 @@ __device__ __forceinline__ float clipped(float g, float factor) {
     return kClip ? __fmul_rn(g, factor) : g;
 }
 
+// Four gradients; the clipped step lets go of the lines that the norm's pass kept in the L2.
+template <bool kClip>
+__device__ __forceinline__ float4 load_grad(const float* p) {
+    if (!kClip) return __ldg(reinterpret_cast<const float4*>(p));
+    const uint4 v = gradnorm::load_hinted(p, gradnorm::l2_policy(false));
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
 template <bool kClip>
 __device__ __forceinline__ void upd(float& p, float g, float& m, float& v, const Group& G, const Table& t,
                                     float factor) {
     adam_element(p, clipped<kClip>(g, factor), m, v, G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
 }
 
+// One tile of kPerBlock elements from `base` on, by kThreads threads.
 template <bool kClip>
-__global__ void __launch_bounds__(kThreads) k_adam(Table t, gradnorm::Clip c) {
-    const float f = kClip ? static_cast<float>(gradnorm::block_factor(c, true)) : 1.f;
-    int gi = 0;
-#pragma unroll 1
-    while (gi + 1 < t.count && static_cast<long long>(blockIdx.x) >= t.g[gi + 1].first_block) ++gi;
-    const Group& G = t.g[gi];
-    const long long base = (static_cast<long long>(blockIdx.x) - G.first_block) * kPerBlock;
+__device__ __forceinline__ void adam_tile(const Group& G, const Table& t, long long base, int thread, float f) {
     if (G.vec) {
 #pragma unroll
         for (int k = 0; k < kPerBlock / (kThreads * kVec); ++k) {
-            const long long e = base + (static_cast<long long>(k) * kThreads + threadIdx.x) * kVec;
+            const long long e = base + (static_cast<long long>(k) * kThreads + thread) * kVec;
             if (e + kVec <= G.n) {
                 float4 p = *reinterpret_cast<const float4*>(G.param + e);
-                const float4 g = __ldg(reinterpret_cast<const float4*>(G.grad + e));
+                const float4 g = load_grad<kClip>(G.grad + e);
                 float4 m = *reinterpret_cast<const float4*>(G.exp_avg + e);
                 float4 v = *reinterpret_cast<const float4*>(G.exp_avg_sq + e);
                 upd<kClip>(p.x, g.x, m.x, v.x, G, t, f);
@@ -82,8 +90,49 @@ __global__ void __launch_bounds__(kThreads) k_adam(Table t, gradnorm::Clip c) {
             }
         }
     } else {
-        for (long long e = base + threadIdx.x; e < base + kPerBlock && e < G.n; e += kThreads)
+        for (long long e = base + thread; e < base + kPerBlock && e < G.n; e += kThreads)
             upd<kClip>(G.param[e], G.grad[e], G.exp_avg[e], G.exp_avg_sq[e], G, t, f);
+    }
+}
+
+// The group that tile `tile` of the launch belongs to.
+template <typename T>
+__device__ __forceinline__ int group_of(const T& t, long long tile) {
+    int gi = 0;
+#pragma unroll 1
+    while (gi + 1 < t.count && tile >= t.g[gi + 1].first_block) ++gi;
+    return gi;
+}
+
+__global__ void __launch_bounds__(kThreads) k_adam(Table t) {
+    const Group& G = t.g[group_of(t, blockIdx.x)];
+    adam_tile<false>(G, t, (static_cast<long long>(blockIdx.x) - G.first_block) * kPerBlock, threadIdx.x, 1.f);
+}
+
+// The clipped step. The last tiles come first: the norm's pass left their gradients in the L2.
+__global__ void __launch_bounds__(kThreads)
+    k_adam_clipped(const __grid_constant__ Table t, const __grid_constant__ gradnorm::Clip c) {
+    const long long tile = gridDim.x - 1u - blockIdx.x;
+    const Group& G = t.g[group_of(t, tile)];
+    gradnorm::wait_for_primary();
+    const float f = static_cast<float>(gradnorm::factor_of(gradnorm::load_norm(c), c.max_norm));
+    adam_tile<true>(G, t, (tile - G.first_block) * kPerBlock, threadIdx.x, f);
+}
+
+// The clipped step of a small model in one launch: every cluster takes the norm of all gradients for itself, then its
+// share of the tiles.
+template <int NORM>
+__global__ void __launch_bounds__(gradnorm::kSmallThreads)
+    k_adam_small(const __grid_constant__ Table t, const __grid_constant__ GradTable grads,
+                 const __grid_constant__ gradnorm::Clip c, long long tiles) {
+    const double norm = gradnorm::cluster_norm<SPLAT_ADAM_MAX_GROUPS, NORM>(grads, 0);
+    if (blockIdx.x == 0 && threadIdx.x == 0) gradnorm::store_norm(c, norm);
+    const float f = static_cast<float>(gradnorm::factor_of(norm, c.max_norm));
+    constexpr int kTeams = gradnorm::kSmallThreads / kThreads;
+    for (long long tile = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / kThreads; tile < tiles;
+         tile += static_cast<long long>(gridDim.x) * kTeams) {
+        const Group& G = t.g[group_of(t, tile)];
+        adam_tile<true>(G, t, (tile - G.first_block) * kPerBlock, threadIdx.x % kThreads, f);
     }
 }
 
@@ -163,7 +212,6 @@ __device__ __forceinline__ void lean_one(const LeanGroup& G, const LeanTable& t,
 // division per four elements, walking from the first element's primitive across the (at most four) primitives
 // they belong to and loading each one's visibility once.
 __device__ __forceinline__ unsigned lean_mask(const LeanGroup& G, const LeanTable& t, long long e) {
-    if (!t.visibility) return (1u << kVec) - 1u;
     long long prim = primitive_of(G, e);
     int r = static_cast<int>(e - prim * G.features);
     bool vis = t.visibility[prim] != 0;
@@ -180,96 +228,162 @@ __device__ __forceinline__ unsigned lean_mask(const LeanGroup& G, const LeanTabl
     return mask;
 }
 
-// Four consecutive elements with vector accesses, `mask` from lean_mask (non-zero): elements of primitives that
-// are not visible keep their parameter and moments.
+// Four consecutive elements from e, read and written with vector accesses.
 template <bool kLowp, bool kClip>
-__device__ __forceinline__ void lean_four(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask,
-                                          float f) {
-    bool on[kVec];
+struct LeanFour {
+    float4 p, g, m4, v4;  // m4, v4: float32 moments
+    uint2 mb, vb;         // bfloat16 moments
+
+    __device__ __forceinline__ void load(const LeanGroup& G, long long e) {
+        p = *reinterpret_cast<const float4*>(G.param + e);
+        g = load_grad<kClip>(G.grad + e);
+        if (kLowp) {
+            mb = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(G.exp_avg) + e);
+            vb = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(G.exp_avg_sq) + e);
+        } else {
+            m4 = *reinterpret_cast<const float4*>(static_cast<const float*>(G.exp_avg) + e);
+            v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(G.exp_avg_sq) + e);
+        }
+    }
+
+    // Updates and stores them; `mask` from lean_mask (non-zero): elements of primitives that are not visible keep
+    // their parameter and moments.
+    __device__ __forceinline__ void update(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask, float f) {
+        float pv[kVec] = {p.x, p.y, p.z, p.w}, gv[kVec] = {g.x, g.y, g.z, g.w}, mv[kVec], vv[kVec];
+        uint32_t mo[2] = {mb.x, mb.y}, vo[2] = {vb.x, vb.y};
+        if (kLowp) {
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) on[k] = (mask >> k) & 1u;
-    float4 p = *reinterpret_cast<const float4*>(G.param + e);
-    const float4 g4 = __ldg(reinterpret_cast<const float4*>(G.grad + e));
-    float pv[kVec] = {p.x, p.y, p.z, p.w}, gv[kVec] = {g4.x, g4.y, g4.z, g4.w}, mv[kVec], vv[kVec];
-    uint2 mb{}, vb{};
-    if (kLowp) {
-        mb = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(G.exp_avg) + e);
-        vb = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(G.exp_avg_sq) + e);
-        const uint32_t mw[2] = {mb.x, mb.y}, vw[2] = {vb.x, vb.y};
+            for (int k = 0; k < kVec; ++k) {
+                mv[k] = bf16_to_float(static_cast<uint16_t>(mo[k >> 1] >> (16 * (k & 1))));
+                vv[k] = bf16_to_float(static_cast<uint16_t>(vo[k >> 1] >> (16 * (k & 1))));
+            }
+        } else {
+            mv[0] = m4.x, mv[1] = m4.y, mv[2] = m4.z, mv[3] = m4.w;
+            vv[0] = v4.x, vv[1] = v4.y, vv[2] = v4.z, vv[3] = v4.w;
+        }
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
-            mv[k] = bf16_to_float(static_cast<uint16_t>(mw[k >> 1] >> (16 * (k & 1))));
-            vv[k] = bf16_to_float(static_cast<uint16_t>(vw[k >> 1] >> (16 * (k & 1))));
-        }
-    } else {
-        const float4 m4 = *reinterpret_cast<const float4*>(static_cast<const float*>(G.exp_avg) + e);
-        const float4 v4 = *reinterpret_cast<const float4*>(static_cast<const float*>(G.exp_avg_sq) + e);
-        mv[0] = m4.x, mv[1] = m4.y, mv[2] = m4.z, mv[3] = m4.w;
-        vv[0] = v4.x, vv[1] = v4.y, vv[2] = v4.z, vv[3] = v4.w;
-    }
-    uint32_t mo[2] = {mb.x, mb.y}, vo[2] = {vb.x, vb.y};
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-        if (!on[k]) continue;
-        adam_element(pv[k], clipped<kClip>(gv[k], f), mv[k], vv[k], G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
-        const float m = mv[k], v = vv[k];
-        if (kLowp) {
-            const uint32_t r1 = lowbias32(static_cast<uint32_t>(e + k) ^ t.seed);
-            const uint32_t r2 = lowbias32(r1);
-            const int sh = 16 * (k & 1);
-            mo[k >> 1] = (mo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(m, r1)) << sh);
-            vo[k >> 1] = (vo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(v, r2)) << sh);
-        }
-    }
-    *reinterpret_cast<float4*>(G.param + e) = make_float4(pv[0], pv[1], pv[2], pv[3]);
-    if (kLowp) {
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(G.exp_avg) + e) = make_uint2(mo[0], mo[1]);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(G.exp_avg_sq) + e) = make_uint2(vo[0], vo[1]);
-    } else {
-        *reinterpret_cast<float4*>(static_cast<float*>(G.exp_avg) + e) = make_float4(mv[0], mv[1], mv[2], mv[3]);
-        *reinterpret_cast<float4*>(static_cast<float*>(G.exp_avg_sq) + e) = make_float4(vv[0], vv[1], vv[2], vv[3]);
-    }
-}
-
-template <bool kLowp, bool kClip>
-__device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, float f) {
-    if (G.vec) {
-        // the visibility of all of this thread's groups of four first, so that their loads overlap one another
-        // instead of each one delaying its group's data loads
-        constexpr int kIters = kPerBlock / (kThreads * kVec);
-        unsigned mask[kIters];
-#pragma unroll
-        for (int k = 0; k < kIters; ++k) {
-            const long long e = base + (static_cast<long long>(k) * kThreads + threadIdx.x) * kVec;
-            mask[k] = e + kVec <= G.n ? lean_mask(G, t, e) : 0u;
-        }
-#pragma unroll
-        for (int k = 0; k < kIters; ++k) {
-            const long long e = base + (static_cast<long long>(k) * kThreads + threadIdx.x) * kVec;
-            if (e + kVec <= G.n) {
-                if (mask[k]) lean_four<kLowp, kClip>(G, t, e, mask[k], f);
-            } else {
-                for (long long j = e; j < G.n; ++j) lean_one<kLowp, kClip>(G, t, j, f);
+            if (!((mask >> k) & 1u)) continue;
+            adam_element(pv[k], clipped<kClip>(gv[k], f), mv[k], vv[k], G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2,
+                         t.eps);
+            if (kLowp) {
+                const uint32_t r1 = lowbias32(static_cast<uint32_t>(e + k) ^ t.seed);
+                const uint32_t r2 = lowbias32(r1);
+                const int sh = 16 * (k & 1);
+                mo[k >> 1] = (mo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(mv[k], r1)) << sh);
+                vo[k >> 1] = (vo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(vv[k], r2)) << sh);
             }
         }
-    } else {
-        for (long long e = base + threadIdx.x; e < base + kPerBlock && e < G.n; e += kThreads)
+        *reinterpret_cast<float4*>(G.param + e) = make_float4(pv[0], pv[1], pv[2], pv[3]);
+        if (kLowp) {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(G.exp_avg) + e) = make_uint2(mo[0], mo[1]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(G.exp_avg_sq) + e) = make_uint2(vo[0], vo[1]);
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(G.exp_avg) + e) = make_float4(mv[0], mv[1], mv[2], mv[3]);
+            *reinterpret_cast<float4*>(static_cast<float*>(G.exp_avg_sq) + e) = make_float4(vv[0], vv[1], vv[2], vv[3]);
+        }
+    }
+};
+
+constexpr int kLeanIters = kPerBlock / (kThreads * kVec);
+constexpr int kLeanList = 32 * kLeanIters;  // groups of four elements that a warp looks at in a tile
+
+// One tile, by kThreads threads whose warps each have kLeanList entries of shared memory at `list`. With a mask, a
+// warp first collects its groups of four that have a visible element (the visibility of all of them is loaded before
+// any is used) and then deals them to its lanes in order: the update is dozens of instructions an element, which the
+// lanes of groups without one would sit through.
+template <bool kLowp, bool kClip>
+__device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, int thread,
+                                           uint16_t* list, float f) {
+    if (!G.vec) {
+        for (long long e = base + thread; e < base + kPerBlock && e < G.n; e += kThreads)
             lean_one<kLowp, kClip>(G, t, e, f);
+        return;
+    }
+    if (t.visibility) {
+        unsigned mask[kLeanIters];
+#pragma unroll
+        for (int k = 0; k < kLeanIters; ++k) {
+            const long long e = base + (static_cast<long long>(k) * kThreads + thread) * kVec;
+            mask[k] = e + kVec <= G.n ? lean_mask(G, t, e) : 0u;
+        }
+        const int lane = thread & 31;
+        int count = 0;
+#pragma unroll
+        for (int k = 0; k < kLeanIters; ++k) {
+            const unsigned some = __ballot_sync(kFullMask, mask[k] != 0u);
+            if (mask[k])
+                list[count + __popc(some & ((1u << lane) - 1u))] =
+                    static_cast<uint16_t>((k * kThreads + thread) << kVec | mask[k]);
+            count += __popc(some);
+        }
+        __syncwarp();
+        for (int j = lane; j < count; j += 64) {
+            const unsigned a = list[j];
+            const bool two = j + 32 < count;
+            const unsigned b = two ? list[j + 32] : a;
+            const long long ea = base + static_cast<long long>(a >> kVec) * kVec;
+            const long long eb = base + static_cast<long long>(b >> kVec) * kVec;
+            LeanFour<kLowp, kClip> x, y;
+            x.load(G, ea);
+            if (two) y.load(G, eb);
+            x.update(G, t, ea, a & ((1u << kVec) - 1u), f);
+            if (two) y.update(G, t, eb, b & ((1u << kVec) - 1u), f);
+        }
+        __syncwarp();  // the list is read before a next tile fills it
+    }
+#pragma unroll
+    for (int k = 0; k < kLeanIters; ++k) {
+        const long long e = base + (static_cast<long long>(k) * kThreads + thread) * kVec;
+        if (e + kVec <= G.n) {
+            if (!t.visibility) {
+                LeanFour<kLowp, kClip> x;
+                x.load(G, e);
+                x.update(G, t, e, (1u << kVec) - 1u, f);
+            }
+        } else {
+            for (long long j = e; j < G.n; ++j) lean_one<kLowp, kClip>(G, t, j, f);
+        }
     }
 }
 
 template <bool kClip>
-__global__ void __launch_bounds__(kThreads) k_adam_lean(LeanTable t, gradnorm::Clip c) {
-    const float f = kClip ? static_cast<float>(gradnorm::block_factor(c, true)) : 1.f;
-    int gi = 0;
-#pragma unroll 1
-    while (gi + 1 < t.count && static_cast<long long>(blockIdx.x) >= t.g[gi + 1].first_block) ++gi;
-    const LeanGroup& G = t.g[gi];
-    const long long base = (static_cast<long long>(blockIdx.x) - G.first_block) * kPerBlock;
+__device__ __forceinline__ void lean_tile(const LeanTable& t, long long tile, int thread, uint16_t* list, float f) {
+    const LeanGroup& G = t.g[group_of(t, tile)];
+    const long long base = (tile - G.first_block) * kPerBlock;
     if (G.lowp)
-        lean_block<true, kClip>(G, t, base, f);
+        lean_block<true, kClip>(G, t, base, thread, list, f);
     else
-        lean_block<false, kClip>(G, t, base, f);
+        lean_block<false, kClip>(G, t, base, thread, list, f);
+}
+
+__global__ void __launch_bounds__(kThreads) k_adam_lean(const __grid_constant__ LeanTable t) {
+    __shared__ uint16_t s_list[kThreads / 32][kLeanList];
+    lean_tile<false>(t, blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], 1.f);
+}
+
+// As k_adam_clipped.
+__global__ void __launch_bounds__(kThreads)
+    k_adam_lean_clipped(const __grid_constant__ LeanTable t, const __grid_constant__ gradnorm::Clip c) {
+    __shared__ uint16_t s_list[kThreads / 32][kLeanList];
+    gradnorm::wait_for_primary();
+    const float f = static_cast<float>(gradnorm::factor_of(gradnorm::load_norm(c), c.max_norm));
+    lean_tile<true>(t, gridDim.x - 1u - blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], f);
+}
+
+// As k_adam_small.
+template <int NORM>
+__global__ void __launch_bounds__(gradnorm::kSmallThreads)
+    k_adam_lean_small(const __grid_constant__ LeanTable t, const __grid_constant__ GradTable grads,
+                      const __grid_constant__ gradnorm::Clip c, long long tiles) {
+    __shared__ uint16_t s_list[gradnorm::kSmallThreads / 32][kLeanList];
+    const double norm = gradnorm::cluster_norm<SPLAT_ADAM_MAX_GROUPS, NORM>(grads, 0);
+    if (blockIdx.x == 0 && threadIdx.x == 0) gradnorm::store_norm(c, norm);
+    const float f = static_cast<float>(gradnorm::factor_of(norm, c.max_norm));
+    constexpr int kTeams = gradnorm::kSmallThreads / kThreads;
+    for (long long tile = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / kThreads; tile < tiles;
+         tile += static_cast<long long>(gridDim.x) * kTeams)
+        lean_tile<true>(t, tile, threadIdx.x % kThreads, s_list[threadIdx.x / 32], f);
 }
 
 }  // namespace adam
@@ -360,26 +474,62 @@ int build_lean_table(const char* what, int count, const adam_lean_group* groups,
     return SPLAT_OK;
 }
 
-// The clip factor's source for the groups' gradients: the caller's norm, or partials enqueued here.
-template <typename G>
-int clip_of(const char* what, int count, const G* groups, int norm_type, double max_norm, float* norm, void* workspace,
-            size_t workspace_bytes, cudaStream_t st, gradnorm::Clip& c) {
+struct Grads {
+    const void* grad[SPLAT_ADAM_MAX_GROUPS];
+    long long n[SPLAT_ADAM_MAX_GROUPS];
+    unsigned char dtype[SPLAT_ADAM_MAX_GROUPS];
+};
+
+// A clipped step: the norm's kernel and the update's, or for a small model one kernel that does both.
+template <typename G, typename T>
+int clipped_step(const char* what, int count, const G* groups, const T& table, long long blocks,
+                 void (*update)(T, gradnorm::Clip),
+                 void (*const (&small)[3])(T, adam::GradTable, gradnorm::Clip, long long), int norm_type,
+                 double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
     const bool given = norm_type == SPLAT_NORM_GIVEN;
     SPLAT_REQUIRE(given || gradnorm::known_norm(norm_type), "%s: unknown norm type %d", what, norm_type);
     SPLAT_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", what);
     SPLAT_REQUIRE(norm, "%s: the norm's buffer is missing", what);
     SPLAT_REQUIRE(given || (workspace && workspace_bytes >= splat_grad_workspace_size(count)),
                   "%s: workspace too small", what);
-    c = {static_cast<const double*>(workspace), 0, norm_type, given, 0, norm, max_norm};
-    if (given) return SPLAT_OK;
-    const void* grads[SPLAT_ADAM_MAX_GROUPS];
-    long long n[SPLAT_ADAM_MAX_GROUPS];
-    unsigned char dtypes[SPLAT_ADAM_MAX_GROUPS] = {};  // SPLAT_F32
-    for (int i = 0; i < count; ++i) {
-        grads[i] = groups[i].grad;
-        n[i] = groups[i].n;
+    if (blocks == 0)  // the norm of nothing is the call's all the same
+        return given ? SPLAT_OK
+                     : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,
+                                       stream);
+    const cudaStream_t st = as_stream(stream);
+    const gradnorm::Clip c{norm, max_norm, 0};
+    if (!given) {
+        Grads list{};  // dtype 0: SPLAT_F32
+        for (int i = 0; i < count; ++i) {
+            list.grad[i] = groups[i].grad;
+            list.n[i] = groups[i].n;
+        }
+        if (gradnorm::is_small(count, list.grad, list.n, list.dtype)) {
+            adam::GradTable grads;
+            gradnorm::fill(grads, 0, count, list.grad, nullptr, list.n, list.dtype);
+            constexpr int kTilesPerCluster =
+                gradnorm::kSmallCluster * (gradnorm::kSmallThreads / adam::kThreads);
+            const long long clusters = std::min<long long>((blocks + kTilesPerCluster - 1) / kTilesPerCluster, 8);
+            cudaError_t e = cudaSuccess;
+            SPLAT_TIMED_LAUNCH("k_adam", st,
+                               (e = gradnorm::launch(small[norm_type],
+                                                     static_cast<unsigned int>(clusters * gradnorm::kSmallCluster),
+                                                     gradnorm::kSmallThreads, st, false, gradnorm::kSmallCluster, table,
+                                                     grads, c, blocks)));
+            SPLAT_CUDA(e);
+            note_launch();
+            return check_launch(what);
+        }
+        SPLAT_TRY(gradnorm::enqueue_norm(count, list.grad, list.n, list.dtype, norm_type,
+                                         static_cast<double*>(workspace), c, true, st));
     }
-    return gradnorm::enqueue_partials(count, grads, n, dtypes, norm_type, static_cast<double*>(workspace), &c.count, st);
+    cudaError_t e = cudaSuccess;
+    SPLAT_TIMED_LAUNCH("k_adam", st,
+                       (e = gradnorm::launch(update, static_cast<unsigned int>(blocks), adam::kThreads, st, !given, 1,
+                                             table, c)));
+    SPLAT_CUDA(e);
+    note_launch();
+    return check_launch(what);
 }
 
 }  // namespace
@@ -393,8 +543,7 @@ int adam_step_multi(int count, const adam_group* groups, int step, double beta1,
     SPLAT_TRY(build_table("adam_step_multi", count, groups, step, beta1, beta2, eps, t, &blocks));
     if (blocks == 0) return SPLAT_OK;
     SPLAT_TIMED_LAUNCH("k_adam", as_stream(stream),
-                       (adam::k_adam<false><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(
-                           t, gradnorm::Clip{})));
+                       (adam::k_adam<<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(t)));
     note_launch();
     return check_launch("adam_step_multi");
 }
@@ -406,8 +555,7 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
     SPLAT_TRY(build_lean_table("adam_step_multi_lean", count, groups, step, beta1, beta2, eps, visibility, n_primitives,
                                t, &blocks));
     if (blocks == 0) return SPLAT_OK;
-    adam::k_adam_lean<false><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(
-        t, gradnorm::Clip{});
+    adam::k_adam_lean<<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(t);
     note_launch();
     return check_launch("adam_step_multi_lean");
 }
@@ -415,41 +563,27 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
 int adam_step_multi_clipped(int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
                             int norm_type, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
                             void* stream) {
+    static void (*const small[3])(adam::Table, adam::GradTable, gradnorm::Clip, long long) = {
+        adam::k_adam_small<SPLAT_NORM_INF>, adam::k_adam_small<SPLAT_NORM_L1>, adam::k_adam_small<SPLAT_NORM_L2>};
     adam::Table t{};
     long long blocks = 0;
     SPLAT_TRY(build_table("adam_step_multi_clipped", count, groups, step, beta1, beta2, eps, t, &blocks));
-    const cudaStream_t st = as_stream(stream);
-    gradnorm::Clip c;
-    SPLAT_TRY(clip_of("adam_step_multi_clipped", count, groups, norm_type, max_norm, norm, workspace, workspace_bytes,
-                      st, c));
-    if (blocks == 0)  // the norm of nothing is the call's all the same
-        return c.given ? SPLAT_OK
-                       : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,
-                                         stream);
-    SPLAT_TIMED_LAUNCH("k_adam", st,
-                       (adam::k_adam<true><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, st>>>(t, c)));
-    note_launch();
-    return check_launch("adam_step_multi_clipped");
+    return clipped_step("adam_step_multi_clipped", count, groups, t, blocks, adam::k_adam_clipped, small, norm_type,
+                        max_norm, norm, workspace, workspace_bytes, stream);
 }
 
 int adam_step_multi_lean_clipped(int count, const adam_lean_group* groups, int step, double beta1, double beta2,
                                  double eps, const int32_t* visibility, long long n_primitives, int norm_type,
                                  double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    static void (*const small[3])(adam::LeanTable, adam::GradTable, gradnorm::Clip, long long) = {
+        adam::k_adam_lean_small<SPLAT_NORM_INF>, adam::k_adam_lean_small<SPLAT_NORM_L1>,
+        adam::k_adam_lean_small<SPLAT_NORM_L2>};
     adam::LeanTable t{};
     long long blocks = 0;
     SPLAT_TRY(build_lean_table("adam_step_multi_lean_clipped", count, groups, step, beta1, beta2, eps, visibility,
                                n_primitives, t, &blocks));
-    const cudaStream_t st = as_stream(stream);
-    gradnorm::Clip c;
-    SPLAT_TRY(clip_of("adam_step_multi_lean_clipped", count, groups, norm_type, max_norm, norm, workspace,
-                      workspace_bytes, st, c));
-    if (blocks == 0)
-        return c.given ? SPLAT_OK
-                       : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,
-                                         stream);
-    adam::k_adam_lean<true><<<static_cast<unsigned int>(blocks), adam::kThreads, 0, st>>>(t, c);
-    note_launch();
-    return check_launch("adam_step_multi_lean_clipped");
+    return clipped_step("adam_step_multi_lean_clipped", count, groups, t, blocks, adam::k_adam_lean_clipped, small,
+                        norm_type, max_norm, norm, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

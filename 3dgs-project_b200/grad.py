@@ -14,8 +14,8 @@ apart), and all can be captured into a CUDA graph.
 from __future__ import annotations
 
 import math
-from array import array
-from contextlib import nullcontext
+from functools import lru_cache
+from typing import NamedTuple
 
 import torch
 
@@ -69,55 +69,81 @@ def _refuse(name: str, tensors: list) -> None:
             raise RuntimeError(f"{name} must be on one device, got {first} and {t.device}")
 
 
-def _described(name: str, tensors: list) -> tuple[bytes, int]:
-    """The tensors' type codes and their device index, or an exception for what the kernels do not take."""
-    try:
-        codes = bytes([_CODES[t.dtype] for t in tensors])
-        devices = {t.get_device() for t in tensors}
-        if len(devices) == 1 and min(devices) >= 0 and all([t.is_contiguous() for t in tensors]):
-            return codes, devices.pop()
-    except (AttributeError, KeyError, RuntimeError):
-        pass
-    _refuse(name, tensors)
-    return codes, tensors[0].get_device()
+_native = None
 
 
-def _listed(name: str, tensors) -> list:
+def _tensors():
+    """The module that reads lists of tensors (csrc/tensor_list.cpp), loaded on first use."""
+    global _native
+    if _native is None:
+        try:
+            from . import _tensors as module
+        except ImportError as e:
+            raise RuntimeError("_tensors.so is not built; run `python 3dgs-project_b200/build.py` "
+                               "(or __graft_entry__.build()) first") from e
+        _native = module
+    return _native
+
+
+class Described(NamedTuple):
+    """A list of tensors as the C ABI takes it."""
+
+    addresses: bytes
+    sizes: bytes
+    codes: bytes
+    contiguous: bool
+    device: int
+    current: bool  # the device is the current one
+    stream: int
+
+    def call(self, function: str, *args) -> None:
+        """The library launches on the current device: makes it the tensors'."""
+        if self.current:
+            L.call(function, *args, self.stream)
+        else:
+            with torch.cuda.device(self.device):
+                L.call(function, *args, self.stream)
+
+
+def describe(tensors: list) -> Described | None:
+    """The list read for the C ABI, or None when the kernels do not take one of its entries."""
+    got = _tensors().describe(tensors)
+    return None if got is None else Described._make(got)
+
+
+def _described(name: str, tensors: list) -> Described:
+    d = describe(tensors)
+    if d is None:
+        _refuse(name, tensors)
+        raise RuntimeError(f"{name} cannot be read as dense CUDA tensors")
+    return d
+
+
+def _listed(tensors) -> list:
     if isinstance(tensors, torch.Tensor):
         return [tensors]
-    return list(tensors)
+    return tensors if isinstance(tensors, (list, tuple)) else list(tensors)
 
 
-def _pointers(tensors: list) -> array:
-    return array("Q", [t.data_ptr() for t in tensors])
+@lru_cache(maxsize=None)
+def _workspace_bytes(launch_tables: int) -> int:
+    return L.query("splat_grad_workspace_size", launch_tables * TABLE)
 
 
-def _sizes(tensors: list) -> array:
-    return array("q", [t.numel() for t in tensors])
-
-
-def _address(a: array) -> int:
-    return a.buffer_info()[0]
-
-
-def on_device(index: int):
-    """The library launches on the current device: makes it the tensors'."""
-    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+TABLE = 1000  # tensors of one launch: the workspace grows by the launch
 
 
 def norm_workspace(count: int, device) -> torch.Tensor:
-    return L.workspace(L.query("splat_grad_workspace_size", count), device)
+    return torch.empty(_workspace_bytes((count + TABLE - 1) // TABLE), dtype=torch.uint8, device=device)
 
 
-def _norm(tensors: list, codes: bytes, index: int, norm: int) -> torch.Tensor:
-    device = tensors[0].device
-    f64 = 3 in codes
+def _norm(d: Described, norm: int, device) -> torch.Tensor:
+    f64 = 3 in d.codes
+    count = len(d.codes)
     out = torch.empty((), dtype=torch.float64 if f64 else torch.float32, device=device)
-    ws = norm_workspace(len(tensors), device)
-    ptrs, sizes = _pointers(tensors), _sizes(tensors)
-    with on_device(index):
-        L.call("splat_grad_norm", len(tensors), _address(ptrs), _address(sizes), codes, norm, out.data_ptr(), f64,
-               ws.data_ptr(), ws.numel(), L.stream_of(out))
+    ws = norm_workspace(count, device)
+    d.call("splat_grad_norm", count, d.addresses, d.sizes, d.codes, norm, out.data_ptr(), f64, ws.data_ptr(),
+           ws.numel())
     return out
 
 
@@ -127,22 +153,20 @@ def _check_finite(norm: torch.Tensor, norm_type) -> None:
                            "error_if_nonfinite=False to go on with it")
 
 
-@torch.no_grad()
 def grad_norm(grads, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """The norm of all elements of the tensors as one vector: 0-d, float32 (float64 when one of them is float64), on
     their device. norm_type: 1, 2 or inf. NaN when an element is NaN. No tensors: 0 on the CPU, as torch's clipping
     gives. error_if_nonfinite raises for an infinite or NaN norm (which waits for the device)."""
     norm = norm_code(norm_type)
-    tensors = _listed("grads", grads)
+    tensors = _listed(grads)
     if not tensors:
         return torch.zeros(())
-    total = _norm(tensors, *_described("grads", tensors), norm)
+    total = _norm(_described("grads", tensors), norm, tensors[0].device)
     if error_if_nonfinite:
         _check_finite(total, norm_type)
     return total
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_norm: torch.Tensor | None = None):
     """(clipped, total_norm): the gradients times min(1, max_norm / (total_norm + 1e-6)), each rounded once to its own
     type. A NaN norm makes them all NaN; an infinite one makes them 0, and NaN where they are infinite.
@@ -152,44 +176,39 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     nothing. total_norm: a norm to clip by in place of the gradients' own (one element, float32 or float64, on their
     device: the norm over all ranks, say); it is returned."""
     norm, limit = norm_code(norm_type), check_max_norm(max_norm)
-    tensors = _listed("grads", grads)
-    outs = None if out is None else _listed("out", out)
+    tensors = _listed(grads)
+    in_place = out is grads
+    outs = None if out is None else tensors if in_place else _listed(out)
     if outs is not None and len(outs) != len(tensors):
         raise RuntimeError(f"out has {len(outs)} tensors for {len(tensors)} gradients")
     if not tensors:
         return [], torch.zeros(()) if total_norm is None else total_norm
-    codes, index = _described("grads", tensors)
+    d = _described("grads", tensors)
     if outs is None:
         outs = [torch.empty_like(t) for t in tensors]
-    elif any([o is not t for o, t in zip(outs, tensors)]):
-        out_codes, out_index = _described("out", outs)
-        if out_codes != codes or out_index != index or [o.shape for o in outs] != [t.shape for t in tensors]:
-            raise RuntimeError("out must have the gradients' shapes, types and device")
-        if [o.stride() for o in outs if o.numel()] != [t.stride() for t in tensors if t.numel()]:
-            raise RuntimeError("out must have the gradients' strides")
+    to = d if in_place else _described("out", outs)
+    if not in_place and (to.device != d.device or not _tensors().same_form(tensors, outs)):
+        raise RuntimeError("out must have the gradients' shapes, types, strides and device")
     device = tensors[0].device
-    f64 = 3 in codes
-    given = total_norm is not None
-    if given:
+    f64 = 3 in d.codes
+    count = len(d.codes)
+    if total_norm is None:
+        read = total_norm = torch.empty((), dtype=torch.float64 if f64 else torch.float32, device=device)
+        ws = norm_workspace(count, device)
+        how, ws_ptr, ws_bytes = norm, ws.data_ptr(), ws.numel()
+    else:
         L.check_cuda("total_norm", total_norm)
         if total_norm.dtype not in (torch.float32, torch.float64) or total_norm.numel() != 1 \
                 or total_norm.device != device:
             raise RuntimeError("total_norm must be one float32 or float64 value on the gradients' device")
-        read = total_norm.double() if f64 else total_norm
+        read = total_norm.detach().double() if f64 else total_norm
         f64 = read.dtype == torch.float64
-        ws_ptr, ws_bytes = None, 0
-    else:
-        read = total_norm = torch.empty((), dtype=torch.float64 if f64 else torch.float32, device=device)
-        ws = norm_workspace(len(tensors), device)
-        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-    ptrs, out_ptrs, sizes = _pointers(tensors), _pointers(outs), _sizes(tensors)
-    with on_device(index):
-        L.call("splat_grad_clip", len(tensors), _address(ptrs), _address(out_ptrs), _address(sizes), codes,
-               NORM_GIVEN if given else norm, limit, read.data_ptr(), f64, ws_ptr, ws_bytes, L.stream_of(tensors[0]))
-    return outs, total_norm
+        how, ws_ptr, ws_bytes = NORM_GIVEN, None, 0
+    d.call("splat_grad_clip", count, d.addresses, to.addresses, d.sizes, d.codes, how, limit, read.data_ptr(), f64,
+           ws_ptr, ws_bytes)
+    return list(outs), total_norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the parameters' gradients in place so that their norm together is at most max_norm, and returns the norm
@@ -197,7 +216,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
     not appear twice. error_if_nonfinite raises for an infinite or NaN norm, before anything is scaled (which waits
     for the device)."""
     norm_code(norm_type), check_max_norm(max_norm)
-    grads = [p.grad for p in _listed("parameters", parameters) if p.grad is not None]
+    grads = [p.grad for p in _listed(parameters) if p.grad is not None]
     if not error_if_nonfinite:
         return clip_grads(grads, max_norm, norm_type, out=grads)[1]
     return clip_grads(grads, max_norm, norm_type, out=grads, total_norm=grad_norm(grads, norm_type, True)
