@@ -8,7 +8,7 @@ round-trips with torch's Adam and with checkpoints written by the reference's tr
 from __future__ import annotations
 
 import ctypes
-import struct
+from contextlib import nullcontext
 
 import torch
 
@@ -230,14 +230,16 @@ class FusedAdam(torch.optim.Adam):
             self.grad_norm = torch.zeros(())
             return None
         if in_step:
-            self.grad_norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-            return norm, self.max_grad_norm, self.grad_norm
+            buffers = gs_grad.scratch(grads[0].get_device(), len(grads))
+            self.grad_norm = buffers[0]
+            return norm, self.max_grad_norm, buffers
         self.grad_norm = gs_grad.grad_norm(grads, self.grad_norm_type)
         return gs_grad.NORM_GIVEN, self.max_grad_norm, self.grad_norm
 
 
 def _launch(lean: bool, groups: list, step: int, betas, eps: float, visibility, device, clip) -> None:
-    """One launch over at most MAX_GROUPS entries; `clip` = (norm code, max_norm, the norm's tensor) or None."""
+    """One launch over at most MAX_GROUPS entries; `clip` = (norm code, max_norm, grad.scratch()'s buffers,
+    or with NORM_GIVEN the norm) or None."""
     arr = ((_LeanGroup if lean else _Group) * len(groups))(*groups)
     args = [len(groups), ctypes.addressof(arr), int(step), float(betas[0]), float(betas[1]), float(eps)]
     if lean:
@@ -247,11 +249,13 @@ def _launch(lean: bool, groups: list, step: int, betas, eps: float, visibility, 
     if clip is None:
         L.call(name, *args, stream)
         return
-    norm_type, max_norm, norm = clip
-    ws = None if norm_type == gs_grad.NORM_GIVEN else gs_grad.norm_workspace(len(groups), device)
+    code, max_norm, norm = clip
+    if code == gs_grad.NORM_GIVEN:
+        norm_ptr, ws_ptr, ws_bytes = norm.data_ptr(), None, 0
+    else:
+        norm_ptr, ws_ptr, ws_bytes = norm[1], norm[3], norm[4]
     with torch.cuda.device(device):
-        L.call(name + "_clipped", *args, norm_type, max_norm, norm.data_ptr(), L.ptr(ws),
-               0 if ws is None else ws.numel(), stream)
+        L.call(name + "_clipped", *args, code, max_norm, norm_ptr, ws_ptr, ws_bytes, stream)
 
 
 def _refuse_groups(groups: list[tuple], lean: bool) -> None:
@@ -272,36 +276,17 @@ def _clipped_step(groups: list[tuple], lean: bool, step: int, betas, eps: float,
                   norm_type) -> torch.Tensor:
     """adam_step / adam_step_lean with max_grad_norm: the buffers of all groups read and checked in one go."""
     code, limit = gs_grad.norm_code(norm_type), gs_grad.check_max_norm(max_grad_norm)
-    count = len(groups)
-    params, grads, exp_avg, exp_avg_sq, lrs = zip(*groups)
-    d = gs_grad.describe([*params, *grads, *exp_avg, *exp_avg_sq])
-    if d is None:
+    read = gs_grad.adam_table(groups, lean)
+    if read is None:
         _refuse_groups(groups, lean)
-    size, kinds = 8 * count, d.codes[2 * count:3 * count]
-    sizes = d.sizes[:size]
-    if not d.contiguous or any(d.codes[:2 * count]) or d.codes[3 * count:] != kinds \
-            or max(kinds) > int(lean) or d.sizes != sizes * 4:
-        _refuse_groups(groups, lean)
-    address = struct.unpack(f"{4 * count}Q", d.addresses)
-    n = struct.unpack(f"{count}q", sizes)
-    used = [a for a, k in zip(address, n) if k]
-    if len(set(used)) != len(used):
-        raise RuntimeError("a parameter appears in two groups")
-    rows = []
-    for k in range(count):
-        rows += address[k::count]
-        rows += (n[k], float(lrs[k]))
-        if lean:
-            rows += (n[k] // max(params[k].shape[0], 1), kinds[k])
-    table = struct.pack(("PPPPqdii" if lean else "PPPPqd") * count, *rows)
-    device = params[0].device
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    ws = gs_grad.norm_workspace(count, device)
-    args = [count, table, int(step), float(betas[0]), float(betas[1]), float(eps)]
+    table, device, current, stream = read
+    norm, norm_ptr, ws, ws_ptr, ws_bytes = gs_grad.scratch(device, len(groups))
+    args = [len(groups), table, int(step), float(betas[0]), float(betas[1]), float(eps)]
     if lean:
         args += [L.ptr(visibility), 0 if visibility is None else visibility.numel()]
-    d.call("adam_step_multi_lean_clipped" if lean else "adam_step_multi_clipped", *args, code, limit, norm.data_ptr(),
-           ws.data_ptr(), ws.numel())
+    with nullcontext() if current else torch.cuda.device(device):
+        L.call("adam_step_multi_lean_clipped" if lean else "adam_step_multi_clipped", *args, code, limit, norm_ptr,
+               ws_ptr, ws_bytes, stream)
     return norm
 
 

@@ -56,7 +56,8 @@ def build_tensors(force: bool = False, verbose: bool = False) -> Path:
            f"-I{Path(nvcc()).resolve().parent.parent / 'include'}", f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch_python"]
     version = (torch_dir / "version.py").read_bytes()
-    digest = hashlib.sha256(src.read_bytes() + version + " ".join([sys.version, *cmd]).encode()).hexdigest()
+    header = (INCLUDE / "splat_b200.h").read_bytes()
+    digest = hashlib.sha256(src.read_bytes() + header + version + " ".join([sys.version, *cmd]).encode()).hexdigest()
     stamp = BUILD / "stamp_tensors"
     if not force and TENSORS.exists() and stamp.exists() and stamp.read_text() == digest:
         return TENSORS

@@ -25,6 +25,8 @@ constexpr int kVec = 4;
 constexpr int kPerBlock = kThreads * kVec * 4;  // 4096 elements per block
 static_assert(kThreads == gradnorm::kTeam, "the small kernels split a block into teams of one tile");
 
+constexpr int kSmallParts = kPerBlock / (kThreads * kVec);
+
 using GradTable = gradnorm::Table<SPLAT_ADAM_MAX_GROUPS>;
 
 struct Group {
@@ -51,30 +53,22 @@ __device__ __forceinline__ float clipped(float g, float factor) {
     return kClip ? __fmul_rn(g, factor) : g;
 }
 
-// Four gradients; the clipped step lets go of the lines that the norm's pass kept in the L2.
-template <bool kClip>
-__device__ __forceinline__ float4 load_grad(const float* p) {
-    if (!kClip) return __ldg(reinterpret_cast<const float4*>(p));
-    const uint4 v = gradnorm::load_hinted(p, gradnorm::l2_policy(false));
-    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-}
-
 template <bool kClip>
 __device__ __forceinline__ void upd(float& p, float g, float& m, float& v, const Group& G, const Table& t,
                                     float factor) {
     adam_element(p, clipped<kClip>(g, factor), m, v, G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
 }
 
-// One tile of kPerBlock elements from `base` on, by kThreads threads.
-template <bool kClip>
+// One tile of kIters x 1024 elements from `base` on, by kThreads threads.
+template <bool kClip, int kIters = kPerBlock / (kThreads * kVec)>
 __device__ __forceinline__ void adam_tile(const Group& G, const Table& t, long long base, int thread, float f) {
     if (G.vec) {
 #pragma unroll
-        for (int k = 0; k < kPerBlock / (kThreads * kVec); ++k) {
+        for (int k = 0; k < kIters; ++k) {
             const long long e = base + (static_cast<long long>(k) * kThreads + thread) * kVec;
             if (e + kVec <= G.n) {
                 float4 p = *reinterpret_cast<const float4*>(G.param + e);
-                const float4 g = load_grad<kClip>(G.grad + e);
+                const float4 g = __ldg(reinterpret_cast<const float4*>(G.grad + e));
                 float4 m = *reinterpret_cast<const float4*>(G.exp_avg + e);
                 float4 v = *reinterpret_cast<const float4*>(G.exp_avg_sq + e);
                 upd<kClip>(p.x, g.x, m.x, v.x, G, t, f);
@@ -90,7 +84,7 @@ __device__ __forceinline__ void adam_tile(const Group& G, const Table& t, long l
             }
         }
     } else {
-        for (long long e = base + thread; e < base + kPerBlock && e < G.n; e += kThreads)
+        for (long long e = base + thread; e < base + kIters * kThreads * kVec && e < G.n; e += kThreads)
             upd<kClip>(G.param[e], G.grad[e], G.exp_avg[e], G.exp_avg_sq[e], G, t, f);
     }
 }
@@ -110,7 +104,7 @@ __global__ void __launch_bounds__(kThreads) k_adam(Table t) {
 }
 
 // The clipped step. The last tiles come first: the norm's pass left their gradients in the L2.
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 5)
     k_adam_clipped(const __grid_constant__ Table t, const __grid_constant__ gradnorm::Clip c) {
     const long long tile = gridDim.x - 1u - blockIdx.x;
     const Group& G = t.g[group_of(t, tile)];
@@ -128,15 +122,20 @@ __global__ void __launch_bounds__(gradnorm::kSmallThreads)
     const double norm = gradnorm::cluster_norm<SPLAT_ADAM_MAX_GROUPS, NORM>(grads, 0);
     if (blockIdx.x == 0 && threadIdx.x == 0) gradnorm::store_norm(c, norm);
     const float f = static_cast<float>(gradnorm::factor_of(norm, c.max_norm));
+    // A quarter of a tile at a time: one vector a thread, as many blocks as that takes.
     constexpr int kTeams = gradnorm::kSmallThreads / kThreads;
-    for (long long tile = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / kThreads; tile < tiles;
-         tile += static_cast<long long>(gridDim.x) * kTeams) {
+    for (long long q = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / kThreads; q < kSmallParts * tiles;
+         q += static_cast<long long>(gridDim.x) * kTeams) {
+        const long long tile = q / kSmallParts;
         const Group& G = t.g[group_of(t, tile)];
-        adam_tile<true>(G, t, (tile - G.first_block) * kPerBlock, threadIdx.x % kThreads, f);
+        const long long base = (tile - G.first_block) * kPerBlock + (q % kSmallParts) * (kThreads * kVec);
+        if (base < G.n) adam_tile<true, 1>(G, t, base, threadIdx.x % kThreads, f);
     }
 }
 
 // ---- lean Adam: visibility mask and bfloat16 moments with stochastic rounding ----
+
+constexpr int kLeanPerBlock = 2 * kPerBlock;  // elements per block
 
 struct LeanGroup {
     float* param;
@@ -148,8 +147,9 @@ struct LeanGroup {
     float bc2_sqrt_rcp;
     long long first_block;
     int features;
+    uint32_t magic;  // ceil(2^32 / features)
     int lowp;
-    int vec;  // 16-byte (fp32 moments) / 8-byte (bf16 moments) accesses possible
+    int vec;  // 16-byte (fp32 moments) / 8-byte (bf16 moments) accesses possible, features at most kMaxFeatures
 };
 
 struct LeanTable {
@@ -208,35 +208,56 @@ __device__ __forceinline__ void lean_one(const LeanGroup& G, const LeanTable& t,
     }
 }
 
-// Which of the four consecutive elements from e belong to visible primitives (bit k for element e + k): one
-// division per four elements, walking from the first element's primitive across the (at most four) primitives
-// they belong to and loading each one's visibility once.
-__device__ __forceinline__ unsigned lean_mask(const LeanGroup& G, const LeanTable& t, long long e) {
-    long long prim = primitive_of(G, e);
-    int r = static_cast<int>(e - prim * G.features);
-    bool vis = t.visibility[prim] != 0;
-    unsigned mask = 0u;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-        mask |= static_cast<unsigned>(vis) << k;
-        if (++r == G.features && k + 1 < kVec) {
-            r = 0;
-            ++prim;
-            vis = t.visibility[prim] != 0;
-        }
+// Finds the primitives of a tile's elements with one division a tile: an element's offset from the first element of
+// the tile's first primitive is below 2^16 (features at most kMaxFeatures), where a multiplication by 2^32 / features,
+// rounded up, divides exactly.
+constexpr int kMaxFeatures = 32768;
+
+struct TilePrimitives {
+    const int32_t* visibility;  // of the tile's first primitive
+    uint32_t first;             // elements of that primitive before the tile
+    uint32_t features, magic;
+
+    __device__ __forceinline__ TilePrimitives(const LeanGroup& G, const int32_t* vis, long long base) {
+        const long long prim = primitive_of(G, base);
+        visibility = vis + prim;
+        features = static_cast<uint32_t>(G.features);
+        first = static_cast<uint32_t>(base - prim * G.features);
+        magic = G.magic;
     }
-    return mask;
-}
+
+    // Which of the four elements from offset `o` of the tile on are of visible primitives (bit k: element o + k). All
+    // four exist.
+    __device__ __forceinline__ unsigned mask(uint32_t o) const {
+        if (features == 1) {
+            unsigned m = 0u;
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) m |= static_cast<unsigned>(visibility[o + k] != 0) << k;
+            return m;
+        }
+        const uint32_t x = first + o, p = __umulhi(x, magic);
+        const uint32_t left = (p + 1u) * features - x;  // elements of primitive p from x on
+        unsigned m = visibility[p] != 0 ? (1u << min(left, 4u)) - 1u : 0u;
+        if (left < 4u) {
+            // elements left ... 3 are of the next primitive, or with 2 features of the next two
+            const uint32_t more = min(left + features, 4u);
+            if (visibility[p + 1u] != 0) m |= ((1u << more) - 1u) & ~((1u << left) - 1u);
+            if (more < 4u && visibility[p + 2u] != 0) m |= 0xFu & ~((1u << more) - 1u);
+        }
+        return m;
+    }
+};
+static_assert(kMaxFeatures + kLeanPerBlock <= 65536, "TilePrimitives divides offsets below 2^16");
 
 // Four consecutive elements from e, read and written with vector accesses.
 template <bool kLowp, bool kClip>
 struct LeanFour {
-    float4 p, g, m4, v4;  // m4, v4: float32 moments
-    uint2 mb, vb;         // bfloat16 moments
+    float4 p, g, m4{}, v4{};  // m4, v4: float32 moments
+    uint2 mb{}, vb{};         // bfloat16 moments
 
     __device__ __forceinline__ void load(const LeanGroup& G, long long e) {
         p = *reinterpret_cast<const float4*>(G.param + e);
-        g = load_grad<kClip>(G.grad + e);
+        g = __ldg(reinterpret_cast<const float4*>(G.grad + e));
         if (kLowp) {
             mb = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(G.exp_avg) + e);
             vb = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(G.exp_avg_sq) + e);
@@ -249,29 +270,32 @@ struct LeanFour {
     // Updates and stores them; `mask` from lean_mask (non-zero): elements of primitives that are not visible keep
     // their parameter and moments.
     __device__ __forceinline__ void update(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask, float f) {
-        float pv[kVec] = {p.x, p.y, p.z, p.w}, gv[kVec] = {g.x, g.y, g.z, g.w}, mv[kVec], vv[kVec];
-        uint32_t mo[2] = {mb.x, mb.y}, vo[2] = {vb.x, vb.y};
-        if (kLowp) {
-#pragma unroll
-            for (int k = 0; k < kVec; ++k) {
-                mv[k] = bf16_to_float(static_cast<uint16_t>(mo[k >> 1] >> (16 * (k & 1))));
-                vv[k] = bf16_to_float(static_cast<uint16_t>(vo[k >> 1] >> (16 * (k & 1))));
-            }
-        } else {
-            mv[0] = m4.x, mv[1] = m4.y, mv[2] = m4.z, mv[3] = m4.w;
-            vv[0] = v4.x, vv[1] = v4.y, vv[2] = v4.z, vv[3] = v4.w;
-        }
+        // All four are computed and the result is chosen, so that their long chains (a square root, a division)
+        // overlap.
+        float pv[kVec] = {p.x, p.y, p.z, p.w};
+        const float gv[kVec] = {g.x, g.y, g.z, g.w};
+        float mv[kVec] = {m4.x, m4.y, m4.z, m4.w}, vv[kVec] = {v4.x, v4.y, v4.z, v4.w};
+        uint32_t mo[2] = {0u, 0u}, vo[2] = {0u, 0u};
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
-            if (!((mask >> k) & 1u)) continue;
-            adam_element(pv[k], clipped<kClip>(gv[k], f), mv[k], vv[k], G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2,
-                         t.eps);
+            const bool on = (mask >> k) & 1u;
+            const int sh = 16 * (k & 1);
+            const uint32_t mw = k < 2 ? mb.x : mb.y, vw = k < 2 ? vb.x : vb.y;
+            float p1 = pv[k], m1 = mv[k], v1 = vv[k];
+            if (kLowp) {
+                m1 = bf16_to_float(static_cast<uint16_t>(mw >> sh));
+                v1 = bf16_to_float(static_cast<uint16_t>(vw >> sh));
+            }
+            adam_element(p1, clipped<kClip>(gv[k], f), m1, v1, G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
+            pv[k] = on ? p1 : pv[k];
             if (kLowp) {
                 const uint32_t r1 = lowbias32(static_cast<uint32_t>(e + k) ^ t.seed);
                 const uint32_t r2 = lowbias32(r1);
-                const int sh = 16 * (k & 1);
-                mo[k >> 1] = (mo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(mv[k], r1)) << sh);
-                vo[k >> 1] = (vo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(vv[k], r2)) << sh);
+                mo[k >> 1] |= on ? static_cast<uint32_t>(float_to_bf16_sr(m1, r1)) << sh : mw & (0xFFFFu << sh);
+                vo[k >> 1] |= on ? static_cast<uint32_t>(float_to_bf16_sr(v1, r2)) << sh : vw & (0xFFFFu << sh);
+            } else {
+                mv[k] = on ? m1 : mv[k];
+                vv[k] = on ? v1 : vv[k];
             }
         }
         *reinterpret_cast<float4*>(G.param + e) = make_float4(pv[0], pv[1], pv[2], pv[3]);
@@ -285,7 +309,7 @@ struct LeanFour {
     }
 };
 
-constexpr int kLeanIters = kPerBlock / (kThreads * kVec);
+constexpr int kLeanIters = kLeanPerBlock / (kThreads * kVec);
 constexpr int kLeanList = 32 * kLeanIters;  // groups of four elements that a warp looks at in a tile
 
 // One tile, by kThreads threads whose warps each have kLeanList entries of shared memory at `list`. With a mask, a
@@ -296,16 +320,17 @@ template <bool kLowp, bool kClip>
 __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, int thread,
                                            uint16_t* list, float f) {
     if (!G.vec) {
-        for (long long e = base + thread; e < base + kPerBlock && e < G.n; e += kThreads)
+        for (long long e = base + thread; e < base + kLeanPerBlock && e < G.n; e += kThreads)
             lean_one<kLowp, kClip>(G, t, e, f);
         return;
     }
     if (t.visibility) {
         unsigned mask[kLeanIters];
+        const TilePrimitives prims(G, t.visibility, base);
 #pragma unroll
         for (int k = 0; k < kLeanIters; ++k) {
-            const long long e = base + (static_cast<long long>(k) * kThreads + thread) * kVec;
-            mask[k] = e + kVec <= G.n ? lean_mask(G, t, e) : 0u;
+            const uint32_t o = static_cast<uint32_t>(k * kThreads + thread) * kVec;
+            mask[k] = base + o + kVec <= G.n ? prims.mask(o) : 0u;
         }
         const int lane = thread & 31;
         int count = 0;
@@ -318,17 +343,12 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
             count += __popc(some);
         }
         __syncwarp();
-        for (int j = lane; j < count; j += 64) {
+        for (int j = lane; j < count; j += 32) {
             const unsigned a = list[j];
-            const bool two = j + 32 < count;
-            const unsigned b = two ? list[j + 32] : a;
-            const long long ea = base + static_cast<long long>(a >> kVec) * kVec;
-            const long long eb = base + static_cast<long long>(b >> kVec) * kVec;
-            LeanFour<kLowp, kClip> x, y;
-            x.load(G, ea);
-            if (two) y.load(G, eb);
-            x.update(G, t, ea, a & ((1u << kVec) - 1u), f);
-            if (two) y.update(G, t, eb, b & ((1u << kVec) - 1u), f);
+            const long long e = base + static_cast<long long>(a >> kVec) * kVec;
+            LeanFour<kLowp, kClip> x;
+            x.load(G, e);
+            x.update(G, t, e, a & ((1u << kVec) - 1u), f);
         }
         __syncwarp();  // the list is read before a next tile fills it
     }
@@ -350,7 +370,7 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
 template <bool kClip>
 __device__ __forceinline__ void lean_tile(const LeanTable& t, long long tile, int thread, uint16_t* list, float f) {
     const LeanGroup& G = t.g[group_of(t, tile)];
-    const long long base = (tile - G.first_block) * kPerBlock;
+    const long long base = (tile - G.first_block) * kLeanPerBlock;
     if (G.lowp)
         lean_block<true, kClip>(G, t, base, thread, list, f);
     else
@@ -462,11 +482,13 @@ int build_lean_table(const char* what, int count, const adam_lean_group* groups,
         bias_corrections(g.lr, beta1, beta2, step, G.step_size, G.bc2_sqrt_rcp);
         G.first_block = blocks;
         G.features = g.features;
+        G.magic = static_cast<uint32_t>(((1ull << 32) + g.features - 1) / g.features);
         G.lowp = g.lowp_moments != 0;
         const uintptr_t moment_align = G.lowp ? 7u : 15u;
         G.vec = ((reinterpret_cast<uintptr_t>(g.param) | reinterpret_cast<uintptr_t>(g.grad)) & 15u) == 0 &&
-                ((reinterpret_cast<uintptr_t>(g.exp_avg) | reinterpret_cast<uintptr_t>(g.exp_avg_sq)) & moment_align) == 0;
-        blocks += (g.n + adam::kPerBlock - 1) / adam::kPerBlock;
+                ((reinterpret_cast<uintptr_t>(g.exp_avg) | reinterpret_cast<uintptr_t>(g.exp_avg_sq)) & moment_align) == 0 &&
+                (!visibility || g.features <= adam::kMaxFeatures);
+        blocks += (g.n + adam::kLeanPerBlock - 1) / adam::kLeanPerBlock;
     }
     t.count = k;
     SPLAT_REQUIRE(blocks < (1ll << 31), "%s: too many elements", what);
@@ -509,7 +531,8 @@ int clipped_step(const char* what, int count, const G* groups, const T& table, l
             gradnorm::fill(grads, 0, count, list.grad, nullptr, list.n, list.dtype);
             constexpr int kTilesPerCluster =
                 gradnorm::kSmallCluster * (gradnorm::kSmallThreads / adam::kThreads);
-            const long long clusters = std::min<long long>((blocks + kTilesPerCluster - 1) / kTilesPerCluster, 8);
+            const long long clusters =
+                std::min<long long>((adam::kSmallParts * blocks + kTilesPerCluster - 1) / kTilesPerCluster, 8);
             cudaError_t e = cudaSuccess;
             SPLAT_TIMED_LAUNCH("k_adam", st,
                                (e = gradnorm::launch(small[norm_type],

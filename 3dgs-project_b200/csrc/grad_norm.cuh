@@ -31,6 +31,7 @@ constexpr int kMaxPartials = 1024;  // of one launch
 constexpr int kSmallCluster = 8;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallChunks = 64;
+constexpr int kSmallTensors = 64;
 
 // Tables of up to 1000 tensors (29 KB of the 32764 bytes a kernel's parameters may take); longer lists take several
 // launches.
@@ -353,7 +354,7 @@ int fill(Table<CAP>& t, int from, int count, const void* const* src, void* const
 
 // A list whose norm takes one launch (also an empty one).
 inline bool is_small(int count, const void* const* grads, const long long* n, const unsigned char* dtypes) {
-    if (count > 128) return false;
+    if (count > kSmallTensors) return false;
     long long chunks = 0;
     for (int i = 0; i < count; ++i)
         if (n[i] > 0) chunks += chunks_of(grads[i], n[i], dtypes[i]);

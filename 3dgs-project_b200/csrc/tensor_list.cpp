@@ -1,5 +1,6 @@
-// tensor_list.cpp - reads a list of tensors for the entry points that take many (gs_b200.grad, the clipped steps of
-// gs_b200.adam): their addresses, sizes and types as packed arrays, in one call from Python.
+// tensor_list.cpp - the Python side's reading of tensors for the entry points that take many (gs_b200.grad, the clipped
+// steps of gs_b200.adam): addresses, sizes and types as the C ABI's arrays, in one call from Python, and the buffers
+// that such a call needs.
 //
 // Asked through Python, a tensor's five properties cost about 0.4 us, which for a few hundred tensors is ten times
 // what the kernels take. This module launches nothing; the kernels stay behind the C ABI.
@@ -7,11 +8,14 @@
 #include <Python.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
 #include <exception>
 #include <vector>
+
+#include "../../include/splat_b200.h"
 
 namespace {
 
@@ -38,8 +42,8 @@ struct Entries {
     }
 };
 
-// describe(list or tuple) -> (addresses uint64, element counts int64, type codes uint8, all contiguous, device index,
-// whether that is the current device, its current stream), the first three as bytes, when every entry is a dense
+// describe(list or tuple) -> (addresses uint64, element counts int64, type codes uint8, device index, whether that is
+// the current device, its current stream), the first three as bytes, when every entry is a dense
 // strided CUDA tensor of a known type, all on one device; otherwise None (the caller then says which is not, and why).
 PyObject* describe(PyObject*, PyObject* seq) {
     const Entries e(seq);
@@ -49,7 +53,6 @@ PyObject* describe(PyObject*, PyObject* seq) {
         std::vector<int64_t> size(e.count);
         std::vector<uint8_t> code(e.count);
         int device = -1;
-        bool contiguous = true;
         for (Py_ssize_t i = 0; i < e.count; ++i) {
             if (!THPVariable_Check(e.items[i])) Py_RETURN_NONE;
             const at::Tensor& t = THPVariable_Unpack(e.items[i]);
@@ -58,19 +61,16 @@ PyObject* describe(PyObject*, PyObject* seq) {
             if (c < 0 || (i > 0 && t.get_device() != device)) Py_RETURN_NONE;
             device = static_cast<int>(t.get_device());
             size[i] = t.numel();
-            if (!t.is_contiguous()) {
-                contiguous = false;
-                if (size[i] > 0 && !t.is_non_overlapping_and_dense()) Py_RETURN_NONE;
-            }
+            if (size[i] > 0 && !t.is_contiguous() && !t.is_non_overlapping_and_dense()) Py_RETURN_NONE;
             code[i] = static_cast<uint8_t>(c);
             address[i] = reinterpret_cast<uint64_t>(t.data_ptr());
         }
         const auto index = static_cast<c10::DeviceIndex>(device);
         const auto stream = reinterpret_cast<unsigned long long>(c10::cuda::getCurrentCUDAStream(index).stream());
-        return Py_BuildValue("(y#y#y#OiOK)", reinterpret_cast<const char*>(address.data()), e.count * Py_ssize_t(8),
+        return Py_BuildValue("(y#y#y#iOK)", reinterpret_cast<const char*>(address.data()), e.count * Py_ssize_t(8),
                              reinterpret_cast<const char*>(size.data()), e.count * Py_ssize_t(8),
-                             reinterpret_cast<const char*>(code.data()), e.count, contiguous ? Py_True : Py_False,
-                             device, c10::cuda::current_device() == index ? Py_True : Py_False, stream);
+                             reinterpret_cast<const char*>(code.data()), e.count, device,
+                             c10::cuda::current_device() == index ? Py_True : Py_False, stream);
     } catch (const std::exception&) {  // a tensor without storage of its own (fake, functional)
         Py_RETURN_NONE;
     }
@@ -98,10 +98,104 @@ PyObject* same_form(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_RETURN_TRUE;
 }
 
+// scratch(device, float64, bytes) -> (a 0-d tensor for a norm, its address, a byte tensor, its address), on the device.
+PyObject* scratch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 3) {
+        PyErr_SetString(PyExc_TypeError, "scratch takes a device, a truth value and a size");
+        return nullptr;
+    }
+    const long device = PyLong_AsLong(args[0]);
+    const int f64 = PyObject_IsTrue(args[1]);
+    const long long bytes = PyLong_AsLongLong(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    try {
+        const auto on = at::TensorOptions().device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+        at::Tensor norm = at::empty({}, on.dtype(f64 ? at::kDouble : at::kFloat));
+        at::Tensor space = at::empty({bytes}, on.dtype(at::kByte));
+        const auto norm_at = reinterpret_cast<unsigned long long>(norm.data_ptr());
+        const auto space_at = reinterpret_cast<unsigned long long>(space.data_ptr());
+        return Py_BuildValue("(NKNK)", THPVariable_Wrap(std::move(norm)), norm_at, THPVariable_Wrap(std::move(space)),
+                             space_at);
+    } catch (const std::exception& e) {  // out of memory
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// adam_table(groups, lean) -> (adam_group or adam_lean_group array as bytes, device index, whether that is the current
+// device, its current stream) for groups (param, grad, exp_avg, exp_avg_sq, lr) of contiguous CUDA tensors of one size
+// on one device: float32, or for the lean table both moments bfloat16. None where a group is not that.
+// A parameter that appears twice raises.
+PyObject* adam_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 2) {
+        PyErr_SetString(PyExc_TypeError, "adam_table takes groups and a truth value");
+        return nullptr;
+    }
+    const Entries groups(args[0]);
+    const int lean = PyObject_IsTrue(args[1]);
+    if (groups.count == 0 || lean < 0) Py_RETURN_NONE;
+    try {
+        std::vector<adam_group> dense(lean ? 0 : groups.count);
+        std::vector<adam_lean_group> sparse(lean ? groups.count : 0);
+        std::vector<const void*> params(groups.count);
+        c10::DeviceIndex device = -1;
+        for (Py_ssize_t i = 0; i < groups.count; ++i) {
+            const Entries g(groups.items[i]);
+            if (g.count != 5) Py_RETURN_NONE;
+            void* at[4];
+            at::ScalarType kind[4];
+            long long n = 0, rows = 1;
+            for (int k = 0; k < 4; ++k) {
+                if (!THPVariable_Check(g.items[k])) Py_RETURN_NONE;
+                const at::Tensor& t = THPVariable_Unpack(g.items[k]);
+                if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous()) Py_RETURN_NONE;
+                if (i == 0 && k == 0) device = t.get_device();
+                if (k == 0) {
+                    n = t.numel();
+                    if (lean && t.dim() == 0) Py_RETURN_NONE;
+                    rows = lean && t.size(0) > 0 ? t.size(0) : 1;
+                }
+                if (t.get_device() != device || t.numel() != n) Py_RETURN_NONE;
+                kind[k] = t.scalar_type();
+                at[k] = t.data_ptr();
+            }
+            const bool low = kind[2] == at::kBFloat16;
+            if (kind[0] != at::kFloat || kind[1] != at::kFloat || kind[2] != kind[3] ||
+                !(kind[2] == at::kFloat || (lean && low)))
+                Py_RETURN_NONE;
+            const double lr = PyFloat_AsDouble(g.items[4]);
+            if (lr == -1.0 && PyErr_Occurred()) return nullptr;
+            params[i] = n > 0 ? at[0] : nullptr;
+            for (Py_ssize_t j = 0; j < i; ++j)
+                if (params[i] && params[i] == params[j]) {
+                    PyErr_SetString(PyExc_RuntimeError, "a parameter appears in two groups");
+                    return nullptr;
+                }
+            if (lean)
+                sparse[i] = {static_cast<float*>(at[0]), static_cast<const float*>(at[1]), at[2], at[3], n, lr,
+                             static_cast<int>(n / rows), low ? 1 : 0};
+            else
+                dense[i] = {static_cast<float*>(at[0]), static_cast<const float*>(at[1]), static_cast<float*>(at[2]),
+                            static_cast<float*>(at[3]), n, lr};
+        }
+        const char* table = lean ? reinterpret_cast<const char*>(sparse.data()) : reinterpret_cast<const char*>(dense.data());
+        const Py_ssize_t size = groups.count * static_cast<Py_ssize_t>(lean ? sizeof(adam_lean_group) : sizeof(adam_group));
+        const auto stream = reinterpret_cast<unsigned long long>(c10::cuda::getCurrentCUDAStream(device).stream());
+        return Py_BuildValue("(y#iOK)", table, size, static_cast<int>(device),
+                             c10::cuda::current_device() == device ? Py_True : Py_False, stream);
+    } catch (const std::exception&) {
+        Py_RETURN_NONE;
+    }
+}
+
 PyMethodDef kMethods[] = {
-    {"describe", describe, METH_O, "describe(tensors) -> (addresses, sizes, codes, contiguous, device, current, stream)"},
+    {"describe", describe, METH_O, "describe(tensors) -> (addresses, sizes, codes, device, current, stream)"},
     {"same_form", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(same_form)), METH_FASTCALL,
      "same_form(a, b) -> shapes, types and strides agree"},
+    {"scratch", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(scratch)), METH_FASTCALL,
+     "scratch(device, float64, bytes) -> (norm, address, workspace, address)"},
+    {"adam_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adam_table)), METH_FASTCALL,
+     "adam_table(groups, lean) -> (table, device, current, stream)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

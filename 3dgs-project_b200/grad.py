@@ -91,7 +91,6 @@ class Described(NamedTuple):
     addresses: bytes
     sizes: bytes
     codes: bytes
-    contiguous: bool
     device: int
     current: bool  # the device is the current one
     stream: int
@@ -125,25 +124,31 @@ def _listed(tensors) -> list:
     return tensors if isinstance(tensors, (list, tuple)) else list(tensors)
 
 
-@lru_cache(maxsize=None)
-def _workspace_bytes(launch_tables: int) -> int:
-    return L.query("splat_grad_workspace_size", launch_tables * TABLE)
-
-
 TABLE = 1000  # tensors of one launch: the workspace grows by the launch
 
 
-def norm_workspace(count: int, device) -> torch.Tensor:
-    return torch.empty(_workspace_bytes((count + TABLE - 1) // TABLE), dtype=torch.uint8, device=device)
+@lru_cache(maxsize=None)
+def _workspace_bytes(tables: int) -> int:
+    return L.query("splat_grad_workspace_size", tables * TABLE)
 
 
-def _norm(d: Described, norm: int, device) -> torch.Tensor:
+def scratch(device: int, count: int, f64: bool = False):
+    """(norm, its address, workspace, its address, its bytes) for a call over `count` tensors; the workspace is to live
+    until the call has returned."""
+    size = _workspace_bytes((count + TABLE - 1) // TABLE)
+    return (*_tensors().scratch(device, f64, size), size)
+
+
+def adam_table(groups: list, lean: bool):
+    """The groups as a clipped step's C call takes them, (table, device, current, stream), or None when it does not."""
+    return _tensors().adam_table(groups, lean)
+
+
+def _norm(d: Described, norm: int) -> torch.Tensor:
     f64 = 3 in d.codes
     count = len(d.codes)
-    out = torch.empty((), dtype=torch.float64 if f64 else torch.float32, device=device)
-    ws = norm_workspace(count, device)
-    d.call("splat_grad_norm", count, d.addresses, d.sizes, d.codes, norm, out.data_ptr(), f64, ws.data_ptr(),
-           ws.numel())
+    out, out_ptr, ws, ws_ptr, ws_bytes = scratch(d.device, count, f64)
+    d.call("splat_grad_norm", count, d.addresses, d.sizes, d.codes, norm, out_ptr, f64, ws_ptr, ws_bytes)
     return out
 
 
@@ -161,7 +166,7 @@ def grad_norm(grads, norm_type: float = 2.0, error_if_nonfinite: bool = False) -
     tensors = _listed(grads)
     if not tensors:
         return torch.zeros(())
-    total = _norm(_described("grads", tensors), norm, tensors[0].device)
+    total = _norm(_described("grads", tensors), norm)
     if error_if_nonfinite:
         _check_finite(total, norm_type)
     return total
@@ -189,23 +194,20 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     to = d if in_place else _described("out", outs)
     if not in_place and (to.device != d.device or not _tensors().same_form(tensors, outs)):
         raise RuntimeError("out must have the gradients' shapes, types, strides and device")
-    device = tensors[0].device
     f64 = 3 in d.codes
     count = len(d.codes)
     if total_norm is None:
-        read = total_norm = torch.empty((), dtype=torch.float64 if f64 else torch.float32, device=device)
-        ws = norm_workspace(count, device)
-        how, ws_ptr, ws_bytes = norm, ws.data_ptr(), ws.numel()
+        total_norm, norm_ptr, ws, ws_ptr, ws_bytes = scratch(d.device, count, f64)
     else:
         L.check_cuda("total_norm", total_norm)
         if total_norm.dtype not in (torch.float32, torch.float64) or total_norm.numel() != 1 \
-                or total_norm.device != device:
+                or total_norm.get_device() != d.device:
             raise RuntimeError("total_norm must be one float32 or float64 value on the gradients' device")
         read = total_norm.detach().double() if f64 else total_norm
         f64 = read.dtype == torch.float64
-        how, ws_ptr, ws_bytes = NORM_GIVEN, None, 0
-    d.call("splat_grad_clip", count, d.addresses, to.addresses, d.sizes, d.codes, how, limit, read.data_ptr(), f64,
-           ws_ptr, ws_bytes)
+        norm, norm_ptr, ws_ptr, ws_bytes = NORM_GIVEN, read.data_ptr(), None, 0
+    d.call("splat_grad_clip", count, d.addresses, to.addresses, d.sizes, d.codes, norm, limit, norm_ptr, f64, ws_ptr,
+           ws_bytes)
     return list(outs), total_norm
 
 
