@@ -198,6 +198,7 @@ struct Span {
           end(n + head),
           first(static_cast<long long>(chunk) * kChunkVecs) {}
     __device__ bool whole() const { return (first > 0 || head == 0) && (first + kChunkVecs) * V <= end; }
+    __device__ bool inside(long long e) const { return e >= head && e + V <= end; }
     // the first element of this thread's k-th vector, counted from the boundary
     __device__ long long element(int k, int thread) const { return (first + k * kTeam + thread) * V; }
 };
@@ -218,17 +219,24 @@ __device__ __forceinline__ void accumulate(const T* src, long long n, uint32_t c
 #pragma unroll
             for (int j = 0; j < V; ++j) add<NORM>(acc, widen(x[k].v[j]));
     } else {
+        // the tensor's first or last chunk: the vectors inside it, all loaded before any is used (zeros add nothing),
+        // then the elements of the one or two that it ends in
+        Vec<T> x[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+            x[k].raw = s.inside(s.element(k, thread)) ? load_hinted(base + s.element(k, thread), policy)
+                                                      : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) add<NORM>(acc, widen(x[k].v[j]));
+#pragma unroll 1
         for (int k = 0; k < kUnroll; ++k) {
             const long long e = s.element(k, thread);
-            if (e >= s.head && e + V <= s.end) {
-                Vec<T> x;
-                x.raw = *reinterpret_cast<const uint4*>(base + e);
-#pragma unroll
-                for (int j = 0; j < V; ++j) add<NORM>(acc, widen(x.v[j]));
-            } else {
-                for (int j = 0; j < V; ++j)
-                    if (e + j >= s.head && e + j < s.end) add<NORM>(acc, widen(base[e + j]));
-            }
+            if (s.inside(e) || e >= s.end || e + V <= s.head) continue;
+#pragma unroll 1
+            for (int j = 0; j < V; ++j)
+                if (e + j >= s.head && e + j < s.end) add<NORM>(acc, widen(base[e + j]));
         }
     }
 }
