@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreads) k_adam_lean(const __grid_constant__ 
 }
 
 // As k_adam_clipped.
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 6)
     k_adam_lean_clipped(const __grid_constant__ LeanTable t, const __grid_constant__ gradnorm::Clip c) {
     __shared__ uint16_t s_list[kThreads / 32][kLeanList];
     gradnorm::wait_for_primary();

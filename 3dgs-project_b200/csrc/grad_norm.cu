@@ -236,6 +236,8 @@ int check_list(const char* what, int count, const void* const* grads, const long
     for (int i = 0; i < count; ++i) {
         SPLAT_REQUIRE(n[i] >= 0, "%s: tensor %d has negative size", what, i);
         SPLAT_REQUIRE(dtypes[i] <= SPLAT_F64, "%s: tensor %d has an unknown type", what, i);
+        // 32 TiB; chunk counts stay in 32 bits
+        SPLAT_REQUIRE(n[i] <= (1ll << 45) / size_of(dtypes[i]), "%s: tensor %d has %lld elements", what, i, n[i]);
         SPLAT_REQUIRE(dtypes[i] != SPLAT_F64 || norm_f64, "%s: tensor %d is float64, the norm is not", what, i);
         if (n[i] == 0) continue;
         SPLAT_REQUIRE(grads[i], "%s: tensor %d has a null buffer", what, i);
@@ -250,12 +252,14 @@ struct Range {
     bool written;
 };
 
-// What is written overlaps nothing else: the outputs one another, or (out of place) any input.
+// What is written overlaps nothing else: the outputs one another, (out of place) any input, or the norm.
 int check_overlap(int count, const void* const* grads, void* const* outs, const long long* n,
-                  const unsigned char* dtypes, bool in_place) {
-    std::unique_ptr<Range[]> s(new (std::nothrow) Range[2 * static_cast<size_t>(count)]);
+                  const unsigned char* dtypes, bool in_place, const Clip& c, bool given) {
+    std::unique_ptr<Range[]> s(new (std::nothrow) Range[2 * static_cast<size_t>(count) + 1]);
     SPLAT_REQUIRE(s, "splat_grad_clip: out of host memory");
     int k = 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(c.norm);
+    s[k++] = {at, at + (c.norm_f64 ? 8u : 4u), !given};
     for (int i = 0; i < count; ++i) {
         if (n[i] == 0) continue;
         const uintptr_t bytes = static_cast<uintptr_t>(n[i]) * size_of(dtypes[i]);
@@ -267,7 +271,7 @@ int check_overlap(int count, const void* const* grads, void* const* outs, const 
     uintptr_t written_to = 0, read_to = 0;
     for (int i = 0; i < k; ++i) {
         SPLAT_REQUIRE(s[i].begin >= written_to && (!s[i].written || s[i].begin >= read_to),
-                      "splat_grad_clip: a tensor that is written overlaps another tensor of the call");
+                      "splat_grad_clip: a tensor that is written overlaps another one of the call");
         uintptr_t& to = s[i].written ? written_to : read_to;
         to = std::max(to, s[i].end);
     }
@@ -323,8 +327,8 @@ int splat_grad_clip(int count, const void* const* grads, void* const* outs, cons
         ++(outs[i] == grads[i] ? same : other);
     }
     SPLAT_REQUIRE(same == 0 || other == 0, "splat_grad_clip: some tensors are clipped in place, others are not");
-    SPLAT_TRY(gradnorm::check_overlap(count, grads, outs, n, dtypes, same > 0));
     const gradnorm::Clip c{norm, max_norm, norm_is_f64};
+    SPLAT_TRY(gradnorm::check_overlap(count, grads, outs, n, dtypes, same > 0, c, given));
     const cudaStream_t st = as_stream(stream);
     if (!given) {
         // the norm of a list without elements (0) is still the call's

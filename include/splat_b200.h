@@ -43,7 +43,7 @@ long long splat_launch_count(void);
  * library records begin_event just before and end_event just after every launch of `kernel`, on the stream it
  * launches on (cudaEvent_t handles created by the caller, passed as void*; NULL events stop the timing). Kernels:
  * "k_preprocess", "k_duplicate", "k_blend" (training and render-only forward), "k_blend_backward",
- * "k_preprocess_backward", "k_adam", "gs2d_k_render" (gs2d forward), "gs2d_k_backward_splat". At most four
+ * "k_preprocess_backward", "k_adam" (the clipped steps' update too), "gs2d_k_render" (gs2d forward), "gs2d_k_backward_splat". At most four
  * kernels at once. The events are re-recorded by every launch: read them before the kernel runs again. */
 int splat_time_kernel(const char* kernel, void* begin_event, void* end_event);
 
@@ -386,10 +386,12 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
 /* ---------------------------------------------------------------------------------------------
  * Global gradient norm, clipping by it, and the Adam steps that clip (no counterpart in the reference).
  *   norm = (sum |g|^p)^(1/p) over every element of every tensor, p = 1 or 2, or max |g|; sums in float64, in an order
- *          fixed by the sizes (the same call gives the same bits); NaN when an element is NaN
+ *          fixed by the sizes (the same call gives the same bits); NaN when an element is NaN; float64 elements beyond
+ *          1e154 square to infinity
  *   f = min(1, max_norm / (norm + 1e-6)), NaN when the norm is; computed in float64 from the rounded norm
  * A list of `count` tensors is given as host arrays: device pointers (aligned to their type, no other alignment
- * needed), element counts, and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements may have null pointers.
+ * needed), element counts (at most 32 TiB), and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements may have
+ * null pointers.
  * The arrays are read during the call only. *norm is device memory: float32, or float64 when norm_is_f64, which a list
  * with a float64 tensor needs.
  * workspace: device scratch of splat_grad_workspace_size(count) bytes, not kept between calls; calls that may run at
@@ -408,7 +410,7 @@ int splat_grad_norm(int count, const void* const* grads, const long long* n, con
                     void* norm, int norm_is_f64, void* workspace, size_t workspace_bytes, void* stream);
 /* outs[i] = grads[i] * f, rounded once to the tensor's type (the product of a 16-bit tensor is taken in float32, that
  * of a float32 one by f rounded to float32). outs[i] == grads[i] for every tensor clips in place (where f = 1 nothing
- * is written), otherwise no output may overlap an input; outputs never overlap one another. */
+ * is written), otherwise no output may overlap an input; outputs never overlap one another or the norm. */
 int splat_grad_clip(int count, const void* const* grads, void* const* outs, const long long* n,
                     const unsigned char* dtypes, int norm_type, double max_norm, void* norm, int norm_is_f64,
                     void* workspace, size_t workspace_bytes, void* stream);

@@ -42,6 +42,8 @@ def _error() -> str:
 @pytest.mark.parametrize("kw,says", [
     (dict(sizes=[-1]), "negative size"),
     (dict(codes=[4]), "unknown type"),
+    (dict(sizes=[1 << 62]), "elements"),
+    (dict(sizes=[(1 << 43) + 1]), "elements"),
     (dict(codes=[3]), "float64"),
     (dict(ptrs=[0]), "null buffer"),
     (dict(ptrs=[P + 2]), "not aligned"),
@@ -72,6 +74,9 @@ def test_norm_refusals(kw, says):
     (dict(ptrs=[P, P], outs=[P, P]), "overlaps"),                # the same tensor twice, in place
     (dict(ptrs=[P, P + 32], outs=[P, P + 32]), "overlaps"),      # tensors that share elements, in place
     (dict(ws=None), "workspace"),
+    (dict(norm=8 * P + 8), "overlaps"),                          # the norm inside an output
+    (dict(norm=2 * P + 8), "overlaps"),                          # written over an input
+    (dict(norm=8 * P + 8, norm_type=3), "overlaps"),             # read from what is written
 ])
 def test_clip_refusals(kw, says):
     args = dict(ptrs=[P, 2 * P], outs=[8 * P, 16 * P], sizes=[16, 16], codes=[0, 0])

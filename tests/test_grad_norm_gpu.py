@@ -351,6 +351,26 @@ def test_clipped_lean_adam_is_clipping_then_the_step(cuda, n, masked):
         same_groups(a, b)
 
 
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 7, 45, 8191, 32768, 33000])
+def test_lean_mask_of_every_width(cuda, width):
+    """The lean steps update the rows that are visible as the dense one does, bit for bit, and no others, whatever the
+    row's width is to the groups of four and to the tile (with and without the clip)."""
+    n = max(3, 50_021 // width)
+    torch.manual_seed(width)
+    for share in (0.0, 0.3, 1.0):
+        vis = (torch.rand(n, device=cuda) < share).int()
+        p, g = torch.randn(n, width, device=cuda), torch.randn(n, width, device=cuda)
+        m, v = torch.randn(n, width, device=cuda), torch.rand(n, width, device=cuda)
+        on = (vis != 0)[:, None]
+        for clip in ({}, {"max_grad_norm": 0.5}):
+            dense = [(p.clone(), g, m.clone(), v.clone(), 1e-2)]
+            lean = copies(dense)
+            A.adam_step(dense, 4, **clip)
+            A.adam_step_lean(lean, 4, vis, **clip)
+            for i, old in ((0, p), (2, m), (3, v)):
+                assert torch.equal(lean[0][i], torch.where(on, dense[0][i], old)), (share, clip, i)
+
+
 def test_clipped_adam_against_the_formula(cuda):
     """One step from zero moments against float64. The factor and the product are off by 3 u together, so m by 4 u and
     v by 8 u; m / sqrt(v) and the other operations add fewer than 16 u, relative to the update."""
@@ -499,6 +519,43 @@ def test_optimizer_is_clip_grad_norm_then_its_step(cuda, count, kw):
         else:
             close_norm(oa.grad_norm, [x.grad for x in a], 2.0)
     assert set(oa.state_dict()) == set(ob.state_dict())
+
+
+def test_sparse_optimizer(cuda):
+    """FusedAdam(sparse, lowp_moment_groups, max_grad_norm) against clip_grad_norm_ and the same optimizer without it,
+    over real forwards (the visibility that the mask comes from)."""
+    sc = scenes.gs3d_test_scene("tiny", seed=2)
+    cam = sc["cameras"][0]
+    names = ("means", "scales", "rotations", "opacities", "sh0", "sh_rest")
+    settings = gs3d.RasterizerSettings(*scenes.settings_tuple(cam, sc["active_sh_bases"], cuda))
+    a = [sc[k].to(cuda).requires_grad_(True) for k in names]
+    b = [t.detach().clone().requires_grad_(True) for t in a]
+    kw = {"sparse": True, "lowp_moment_groups": ("g5",)}
+    oa, ob = make_opt(a, max_grad_norm=1e-3, **kw), make_opt(b, **kw)
+    try:
+        for _ in range(3):
+            img = gs3d.diff_rasterize(*a, torch.empty(0), settings)
+            ((img - 0.5) ** 2).mean().backward()
+            for x, y in zip(a, b):
+                y.grad = x.grad.clone()
+            want = G.clip_grad_norm_(b, 1e-3)
+            oa.step()
+            ob.step()
+            assert torch.equal(oa.grad_norm, want)
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+            assert all(torch.equal(oa.state[x]["exp_avg"], ob.state[y]["exp_avg"]) for x, y in zip(a, b))
+            oa.zero_grad()
+    finally:
+        gs3d._Rasterize.track_visibility = False
+
+
+def test_calls_for_another_device_than_the_current_one(cuda):
+    """The guard that a call takes when its tensors' device is not the current one."""
+    g = torch.randn(1000, device=cuda)
+    d = G.describe([g])._replace(current=False)
+    out, out_ptr, ws, ws_ptr, ws_bytes = G.scratch(0, 1)
+    d.call("splat_grad_norm", 1, d.addresses, d.sizes, d.codes, 2, out_ptr, 0, ws_ptr, ws_bytes)
+    assert torch.equal(out, G.grad_norm([g]))
 
 
 def test_training_together(cuda):
