@@ -18,8 +18,12 @@ constexpr int kNormThreads = 512;
 constexpr int kNormBlocks = 4;  // per SM
 constexpr uint32_t kKeepChunks = 4096;  // 64 MiB of the 126 MB L2
 constexpr int kScaleThreads = kTeam;
-constexpr int kScaleChunks = 1;         // per block
-constexpr int kScaleChunksInPlace = 8;  // per block, where most calls write nothing
+// Out of place a block scales one chunk: a resident grid that loops took 84 us where this takes 72 (1M Gaussians, 236 MB
+// read and written). In place most calls find a factor of 1 and end there, and blocks that only end cost time too: with
+// 8 chunks a block the call over 3M Gaussians takes 108.5 us when nothing changes and the scaling 225 us when something
+// does; with 1 it is 127.9 when nothing changes, with 32 the scaling takes 235.
+constexpr unsigned int kScaleChunksInPlace = 8;
+constexpr unsigned int kScaleBlocks = 8;  // per SM, that a short list is spread over all the same
 
 __device__ __forceinline__ float scaled(float g, double f) { return g * static_cast<float>(f); }
 __device__ __forceinline__ double scaled(double g, double f) { return g * f; }
@@ -214,8 +218,9 @@ int scale_all(int count, const void* const* grads, void* const* outs, const long
     for (int i = 0; i < count;) {
         i = fill(t, i, count, grads, outs, n, dtypes);
         if (t.count == 0) break;
-        const unsigned int per_block = in_place ? kScaleChunksInPlace : kScaleChunks;
-        const unsigned int grid = std::min(t.chunks / per_block + (t.chunks % per_block != 0), 0x7fffffffu);
+        unsigned int grid = t.chunks;
+        if (in_place) grid = std::max(div_up(grid, kScaleChunksInPlace), std::min(grid, kScaleBlocks * sm_count()));
+        grid = std::min(grid, 0x7fffffffu);
         SPLAT_CUDA(launch(k_clip_scale<CAP>, grid, kScaleThreads, st, dependent, 1, t, c, in_place));
         dependent = false;
         note_launch();
