@@ -135,8 +135,6 @@ __global__ void __launch_bounds__(gradnorm::kSmallThreads)
 
 // ---- lean Adam: visibility mask and bfloat16 moments with stochastic rounding ----
 
-constexpr int kLeanPerBlock = 2 * kPerBlock;  // elements per block
-
 struct LeanGroup {
     float* param;
     const float* grad;
@@ -247,7 +245,7 @@ struct TilePrimitives {
         return m;
     }
 };
-static_assert(kMaxFeatures + kLeanPerBlock <= 65536, "TilePrimitives divides offsets below 2^16");
+static_assert(kMaxFeatures + kPerBlock <= 65536, "TilePrimitives divides offsets below 2^16");
 
 // Four consecutive elements from e, read and written with vector accesses.
 template <bool kLowp, bool kClip>
@@ -270,32 +268,25 @@ struct LeanFour {
     // Updates and stores them; `mask` from lean_mask (non-zero): elements of primitives that are not visible keep
     // their parameter and moments.
     __device__ __forceinline__ void update(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask, float f) {
-        // All four are computed and the result is chosen, so that their long chains (a square root, a division)
-        // overlap.
         float pv[kVec] = {p.x, p.y, p.z, p.w};
         const float gv[kVec] = {g.x, g.y, g.z, g.w};
         float mv[kVec] = {m4.x, m4.y, m4.z, m4.w}, vv[kVec] = {v4.x, v4.y, v4.z, v4.w};
-        uint32_t mo[2] = {0u, 0u}, vo[2] = {0u, 0u};
+        uint32_t mo[2] = {mb.x, mb.y}, vo[2] = {vb.x, vb.y};
 #pragma unroll
         for (int k = 0; k < kVec; ++k) {
-            const bool on = (mask >> k) & 1u;
+            if (!((mask >> k) & 1u)) continue;
             const int sh = 16 * (k & 1);
-            const uint32_t mw = k < 2 ? mb.x : mb.y, vw = k < 2 ? vb.x : vb.y;
-            float p1 = pv[k], m1 = mv[k], v1 = vv[k];
             if (kLowp) {
-                m1 = bf16_to_float(static_cast<uint16_t>(mw >> sh));
-                v1 = bf16_to_float(static_cast<uint16_t>(vw >> sh));
+                mv[k] = bf16_to_float(static_cast<uint16_t>(mo[k >> 1] >> sh));
+                vv[k] = bf16_to_float(static_cast<uint16_t>(vo[k >> 1] >> sh));
             }
-            adam_element(p1, clipped<kClip>(gv[k], f), m1, v1, G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2, t.eps);
-            pv[k] = on ? p1 : pv[k];
+            adam_element(pv[k], clipped<kClip>(gv[k], f), mv[k], vv[k], G.step_size, G.bc2_sqrt_rcp, t.beta1, t.beta2,
+                         t.eps);
             if (kLowp) {
                 const uint32_t r1 = lowbias32(static_cast<uint32_t>(e + k) ^ t.seed);
                 const uint32_t r2 = lowbias32(r1);
-                mo[k >> 1] |= on ? static_cast<uint32_t>(float_to_bf16_sr(m1, r1)) << sh : mw & (0xFFFFu << sh);
-                vo[k >> 1] |= on ? static_cast<uint32_t>(float_to_bf16_sr(v1, r2)) << sh : vw & (0xFFFFu << sh);
-            } else {
-                mv[k] = on ? m1 : mv[k];
-                vv[k] = on ? v1 : vv[k];
+                mo[k >> 1] = (mo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(mv[k], r1)) << sh);
+                vo[k >> 1] = (vo[k >> 1] & ~(0xFFFFu << sh)) | (static_cast<uint32_t>(float_to_bf16_sr(vv[k], r2)) << sh);
             }
         }
         *reinterpret_cast<float4*>(G.param + e) = make_float4(pv[0], pv[1], pv[2], pv[3]);
@@ -309,7 +300,7 @@ struct LeanFour {
     }
 };
 
-constexpr int kLeanIters = kLeanPerBlock / (kThreads * kVec);
+constexpr int kLeanIters = kPerBlock / (kThreads * kVec);
 constexpr int kLeanList = 32 * kLeanIters;  // groups of four elements that a warp looks at in a tile
 
 // One tile, by kThreads threads whose warps each have kLeanList entries of shared memory at `list`. With a mask, a
@@ -320,7 +311,7 @@ template <bool kLowp, bool kClip>
 __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, int thread,
                                            uint16_t* list, float f) {
     if (!G.vec) {
-        for (long long e = base + thread; e < base + kLeanPerBlock && e < G.n; e += kThreads)
+        for (long long e = base + thread; e < base + kPerBlock && e < G.n; e += kThreads)
             lean_one<kLowp, kClip>(G, t, e, f);
         return;
     }
@@ -343,6 +334,7 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
             count += __popc(some);
         }
         __syncwarp();
+#pragma unroll 1
         for (int j = lane; j < count; j += 32) {
             const unsigned a = list[j];
             const long long e = base + static_cast<long long>(a >> kVec) * kVec;
@@ -370,7 +362,7 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
 template <bool kClip>
 __device__ __forceinline__ void lean_tile(const LeanTable& t, long long tile, int thread, uint16_t* list, float f) {
     const LeanGroup& G = t.g[group_of(t, tile)];
-    const long long base = (tile - G.first_block) * kLeanPerBlock;
+    const long long base = (tile - G.first_block) * kPerBlock;
     if (G.lowp)
         lean_block<true, kClip>(G, t, base, thread, list, f);
     else
@@ -383,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) k_adam_lean(const __grid_constant__ 
 }
 
 // As k_adam_clipped.
-__global__ void __launch_bounds__(kThreads, 6)
+__global__ void __launch_bounds__(kThreads)
     k_adam_lean_clipped(const __grid_constant__ LeanTable t, const __grid_constant__ gradnorm::Clip c) {
     __shared__ uint16_t s_list[kThreads / 32][kLeanList];
     gradnorm::wait_for_primary();
@@ -488,7 +480,7 @@ int build_lean_table(const char* what, int count, const adam_lean_group* groups,
         G.vec = ((reinterpret_cast<uintptr_t>(g.param) | reinterpret_cast<uintptr_t>(g.grad)) & 15u) == 0 &&
                 ((reinterpret_cast<uintptr_t>(g.exp_avg) | reinterpret_cast<uintptr_t>(g.exp_avg_sq)) & moment_align) == 0 &&
                 (!visibility || g.features <= adam::kMaxFeatures);
-        blocks += (g.n + adam::kLeanPerBlock - 1) / adam::kLeanPerBlock;
+        blocks += (g.n + adam::kPerBlock - 1) / adam::kPerBlock;
     }
     t.count = k;
     SPLAT_REQUIRE(blocks < (1ll << 31), "%s: too many elements", what);
