@@ -26,15 +26,18 @@ constexpr int kChunkBytes = kChunkVecs * kVecBytes;
 
 constexpr int kMaxPartials = 1024;  // of one launch
 
-// Lists of at most kSmallChunks chunks take one launch: a cluster reads them all and adds its blocks' sums through
-// distributed shared memory.
+// Lists of at most kSmallChunks chunks (1 MiB) take one launch: a cluster reads them all and adds its blocks' sums
+// through distributed shared memory. Eight SMs are slower than all of them on the longer of these lists, but each launch
+// saved is 3 us of the host's time. The norm of 43 chunks (3000 3D Gaussians): 5.0 us on the device and 9.8 us a call,
+// against 3.5 and 12.7 in two launches. At 86 chunks clipping takes 12.3 us on the device and 16.0 a call, against 6.3
+// and 17.4 in three: there the device has caught up with the host.
 constexpr int kSmallCluster = 8;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallChunks = 64;
 constexpr int kSmallTensors = 64;
 
-// Tables of up to 1000 tensors (29 KB of the 32764 bytes a kernel's parameters may take); longer lists take several
-// launches.
+// Tables of up to 1000 tensors (29 KB of the 32764 bytes that a kernel's parameters may take); longer lists take
+// several launches.
 constexpr int kTableMax = 1000;
 
 template <int CAP>
@@ -162,7 +165,7 @@ __device__ __forceinline__ void add(double& acc, double g) {
         acc = max_nan(acc, fabs(g));
 }
 
-// A 16-byte load whose line the L2 evicts last (`keep`) or first.
+// A 16-byte load with an L2 policy of l2_policy(): the line is evicted last (`keep`) or first.
 __device__ __forceinline__ uint4 load_hinted(const void* p, uint64_t policy) {
     uint4 v;
     asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
