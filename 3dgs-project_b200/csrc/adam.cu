@@ -310,28 +310,28 @@ constexpr int kLeanList = 32 * kLeanIters;  // groups of four elements that a wa
 // warp first collects its groups of four that have a visible element (the visibility of all of them is loaded before
 // any is used) and then deals them to its lanes in order: the update is dozens of instructions an element, which the
 // lanes of groups without one would sit through. Measured on 3M Gaussians with bfloat16 SH moments, against each thread
-// updating its own groups: 51% visible at random 570 us (605), visible in long runs 407 (403), without a mask, where
-// nothing is collected, 590 (606). Not unrolled: two groups in flight a thread took 638 us at random.
-template <bool kLowp, bool kClip>
+// updating its own groups: 51% visible at random 574 us (611), visible in long runs 404 (405), without a mask, where
+// nothing is collected, 590 (615). Not unrolled: two groups in flight a thread took 638 us at random.
+template <bool kLowp, bool kClip, bool kMasked, int kIters>
 __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, int thread,
                                            uint16_t* list, float f) {
     if (!G.vec) {
-        for (long long e = base + thread; e < base + kPerBlock && e < G.n; e += kThreads)
+        for (long long e = base + thread; e < base + kIters * kThreads * kVec && e < G.n; e += kThreads)
             lean_one<kLowp, kClip>(G, t, e, f);
         return;
     }
-    if (t.visibility) {
-        unsigned mask[kLeanIters];
+    if (kMasked) {
+        unsigned mask[kIters];
         const TilePrimitives prims(G, t.visibility, base);
 #pragma unroll
-        for (int k = 0; k < kLeanIters; ++k) {
+        for (int k = 0; k < kIters; ++k) {
             const uint32_t o = static_cast<uint32_t>(k * kThreads + thread) * kVec;
             mask[k] = base + o + kVec <= G.n ? prims.mask(o) : 0u;
         }
         const int lane = thread & 31;
         int count = 0;
 #pragma unroll
-        for (int k = 0; k < kLeanIters; ++k) {
+        for (int k = 0; k < kIters; ++k) {
             const unsigned some = __ballot_sync(kFullMask, mask[k] != 0u);
             if (mask[k])
                 list[count + __popc(some & ((1u << lane) - 1u))] =
@@ -350,10 +350,10 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
         __syncwarp();  // the list is read before a next tile fills it
     }
 #pragma unroll
-    for (int k = 0; k < kLeanIters; ++k) {
+    for (int k = 0; k < kIters; ++k) {
         const long long e = base + (static_cast<long long>(k) * kThreads + thread) * kVec;
         if (e + kVec <= G.n) {
-            if (!t.visibility) {
+            if (!kMasked) {
                 LeanFour<kLowp, kClip> x;
                 x.load(G, e);
                 x.update(G, t, e, (1u << kVec) - 1u, f);
@@ -364,34 +364,42 @@ __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& 
     }
 }
 
-template <bool kClip>
-__device__ __forceinline__ void lean_tile(const LeanTable& t, long long tile, int thread, uint16_t* list, float f) {
+// Part `part` (of kIters x 1024 elements) of a tile; without one, all of it.
+template <bool kClip, bool kMasked, int kIters = kLeanIters>
+__device__ __forceinline__ void lean_tile(const LeanTable& t, long long tile, int thread, uint16_t* list, float f,
+                                          int part = 0) {
     const LeanGroup& G = t.g[group_of(t, tile)];
-    const long long base = (tile - G.first_block) * kPerBlock;
+    const long long base = (tile - G.first_block) * kPerBlock + part * (kIters * kThreads * kVec);
+    if (base >= G.n) return;
     if (G.lowp)
-        lean_block<true, kClip>(G, t, base, thread, list, f);
+        lean_block<true, kClip, kMasked, kIters>(G, t, base, thread, list, f);
     else
-        lean_block<false, kClip>(G, t, base, thread, list, f);
+        lean_block<false, kClip, kMasked, kIters>(G, t, base, thread, list, f);
 }
 
+// kMasked: there is a visibility mask.
+template <bool kMasked>
 __global__ void __launch_bounds__(kThreads) k_adam_lean(const __grid_constant__ LeanTable t) {
     __shared__ uint16_t s_list[kThreads / 32][kLeanList];
-    lean_tile<false>(t, blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], 1.f);
+    lean_tile<false, kMasked>(t, blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], 1.f);
 }
 
-// As k_adam_clipped. 1M Gaussians of which 35% are visible, at random: 175 us after the norm's 33, 754 MB from and to
+// As k_adam_clipped. 1M Gaussians of which 35% are visible, at random: 171 us after the norm's 35, 754 MB from and to
 // HBM, more than the visible elements' 370 MB because rows of 12 to 180 bytes share their 32-byte sectors. 59% of the
 // issue slots are busy beside 4.2 TB/s, and neither more warps nor loads ahead of the update made it faster.
-__global__ void __launch_bounds__(kThreads)
+// With the mask six blocks an SM are faster than five (206 us against 219, the norm included), without it slower (3M
+// Gaussians in float32 773 us against 733).
+template <bool kMasked>
+__global__ void __launch_bounds__(kThreads, kMasked ? 6 : 1)
     k_adam_lean_clipped(const __grid_constant__ LeanTable t, const __grid_constant__ gradnorm::Clip c) {
     __shared__ uint16_t s_list[kThreads / 32][kLeanList];
     gradnorm::wait_for_primary();
     const float f = static_cast<float>(gradnorm::factor_of(gradnorm::load_norm(c), c.max_norm));
-    lean_tile<true>(t, gridDim.x - 1u - blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], f);
+    lean_tile<true, kMasked>(t, gridDim.x - 1u - blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], f);
 }
 
 // As k_adam_small.
-template <int NORM>
+template <int NORM, bool kMasked>
 __global__ void __launch_bounds__(gradnorm::kSmallThreads)
     k_adam_lean_small(const __grid_constant__ LeanTable t, const __grid_constant__ GradTable grads,
                       const __grid_constant__ gradnorm::Clip c, long long tiles) {
@@ -400,9 +408,10 @@ __global__ void __launch_bounds__(gradnorm::kSmallThreads)
     if (blockIdx.x == 0 && threadIdx.x == 0) gradnorm::store_norm(c, norm);
     const float f = static_cast<float>(gradnorm::factor_of(norm, c.max_norm));
     constexpr int kTeams = gradnorm::kSmallThreads / kThreads;
-    for (long long tile = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / kThreads; tile < tiles;
-         tile += static_cast<long long>(gridDim.x) * kTeams)
-        lean_tile<true>(t, tile, threadIdx.x % kThreads, s_list[threadIdx.x / 32], f);
+    for (long long q = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / kThreads; q < kSmallParts * tiles;
+         q += static_cast<long long>(gridDim.x) * kTeams)
+        lean_tile<true, kMasked, 1>(t, q / kSmallParts, threadIdx.x % kThreads, s_list[threadIdx.x / 32], f,
+                                    static_cast<int>(q % kSmallParts));
 }
 
 }  // namespace adam
@@ -577,7 +586,8 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
     SPLAT_TRY(build_lean_table("adam_step_multi_lean", count, groups, step, beta1, beta2, eps, visibility, n_primitives,
                                t, &blocks));
     if (blocks == 0) return SPLAT_OK;
-    adam::k_adam_lean<<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(t);
+    const auto kernel = visibility ? adam::k_adam_lean<true> : adam::k_adam_lean<false>;
+    kernel<<<static_cast<unsigned int>(blocks), adam::kThreads, 0, as_stream(stream)>>>(t);
     note_launch();
     return check_launch("adam_step_multi_lean");
 }
@@ -597,15 +607,20 @@ int adam_step_multi_clipped(int count, const adam_group* groups, int step, doubl
 int adam_step_multi_lean_clipped(int count, const adam_lean_group* groups, int step, double beta1, double beta2,
                                  double eps, const int32_t* visibility, long long n_primitives, int norm_type,
                                  double max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
-    static void (*const small[3])(adam::LeanTable, adam::GradTable, gradnorm::Clip, long long) = {
-        adam::k_adam_lean_small<SPLAT_NORM_INF>, adam::k_adam_lean_small<SPLAT_NORM_L1>,
-        adam::k_adam_lean_small<SPLAT_NORM_L2>};
+    using Small = void (*)(adam::LeanTable, adam::GradTable, gradnorm::Clip, long long);
+    static const Small small[2][3] = {
+        {adam::k_adam_lean_small<SPLAT_NORM_INF, false>, adam::k_adam_lean_small<SPLAT_NORM_L1, false>,
+         adam::k_adam_lean_small<SPLAT_NORM_L2, false>},
+        {adam::k_adam_lean_small<SPLAT_NORM_INF, true>, adam::k_adam_lean_small<SPLAT_NORM_L1, true>,
+         adam::k_adam_lean_small<SPLAT_NORM_L2, true>}};
+    const bool masked = visibility != nullptr;
     adam::LeanTable t{};
     long long blocks = 0;
     SPLAT_TRY(build_lean_table("adam_step_multi_lean_clipped", count, groups, step, beta1, beta2, eps, visibility,
                                n_primitives, t, &blocks));
-    return clipped_step("adam_step_multi_lean_clipped", count, groups, t, blocks, adam::k_adam_lean_clipped, small,
-                        norm_type, max_norm, norm, workspace, workspace_bytes, stream);
+    const auto update = masked ? adam::k_adam_lean_clipped<true> : adam::k_adam_lean_clipped<false>;
+    return clipped_step("adam_step_multi_lean_clipped", count, groups, t, blocks, update, small[masked], norm_type,
+                        max_norm, norm, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"
