@@ -268,7 +268,7 @@ struct LeanFour {
         }
     }
 
-    // Updates and stores them; `mask` from lean_mask (non-zero): elements of primitives that are not visible keep
+    // Updates and stores them; `mask` from TilePrimitives (non-zero): elements of primitives that are not visible keep
     // their parameter and moments.
     __device__ __forceinline__ void update(const LeanGroup& G, const LeanTable& t, long long e, unsigned mask, float f) {
         float pv[kVec] = {p.x, p.y, p.z, p.w};
@@ -384,9 +384,9 @@ __global__ void __launch_bounds__(kThreads) k_adam_lean(const __grid_constant__ 
     lean_tile<false, kMasked>(t, blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], 1.f);
 }
 
-// As k_adam_clipped. 1M Gaussians of which 35% are visible, at random: 171 us after the norm's 35, 754 MB from and to
-// HBM, more than the visible elements' 370 MB because rows of 12 to 180 bytes share their 32-byte sectors. 59% of the
-// issue slots are busy beside 4.2 TB/s, and neither more warps nor loads ahead of the update made it faster.
+// As k_adam_clipped. 1M Gaussians of which 35% are visible, at random: 171 us after the norm's 35, 753 MB from and to
+// HBM, more than the visible elements' 370 MB because rows of 12 to 180 bytes share their 32-byte sectors. 62% of the
+// issue slots are busy beside 4.5 TB/s, and loads ahead of the update made it slower.
 // With the mask six blocks an SM are faster than five (206 us against 219, the norm included), without it slower (3M
 // Gaussians in float32 773 us against 733).
 template <bool kMasked>
@@ -519,9 +519,10 @@ int clipped_step(const char* what, int count, const G* groups, const T& table, l
     const bool given = norm_type == SPLAT_NORM_GIVEN;
     SPLAT_REQUIRE(given || gradnorm::known_norm(norm_type), "%s: unknown norm type %d", what, norm_type);
     SPLAT_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", what);
-    SPLAT_REQUIRE(norm, "%s: the norm's buffer is missing", what);
-    SPLAT_REQUIRE(given || (workspace && workspace_bytes >= splat_grad_workspace_size(count)),
-                  "%s: workspace too small", what);
+    SPLAT_REQUIRE(gradnorm::aligned(norm, false), "%s: the norm's buffer is missing or not aligned", what);
+    SPLAT_REQUIRE(
+        given || (gradnorm::aligned(workspace, true) && workspace_bytes >= splat_grad_workspace_size(count)),
+        "%s: workspace too small or not aligned", what);
     if (blocks == 0)  // the norm of nothing is the call's all the same
         return given ? SPLAT_OK
                      : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,

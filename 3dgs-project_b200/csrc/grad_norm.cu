@@ -6,8 +6,8 @@
 // chunks of 16 KiB from the 16-byte boundary at or before their first element, so that all but the first and the last
 // 16 bytes of a tensor move as 16-byte vectors wherever it starts.
 //
-// The norm reads everything once and is bound by HBM: 105 us for the 708 MB of 3M Gaussians' gradients (6.7 TB/s, 1.02
-// of the measured copy rate). Squares are added in float64, which keeps float32's whole range (a square of 1e-25 or
+// The norm reads everything once and is bound by HBM: 103 us for the 708 MB of 3M Gaussians' gradients (6.9 TB/s, 1.05
+// of the measured copy rate; with lines that leave the L2 first, as a call that reads on wants them, 105). Squares are added in float64, which keeps float32's whole range (a square of 1e-25 or
 // 1e25 leaves it) and every bit of the result; it costs a conversion and a float64 multiply-add an element, hidden
 // behind the loads at 32 registers and all 64 warps of an SM (46 registers, for looking the next chunk up while this
 // one loads, cost 1% on 3M Gaussians and 13% on a ragged 16-bit list). Teams take every teams-th chunk: neighbouring
@@ -77,7 +77,7 @@ __device__ __forceinline__ void scale_chunk(const T* src, T* dst, long long n, u
     const bool vec = ((reinterpret_cast<uintptr_t>(src) ^ reinterpret_cast<uintptr_t>(dst)) & (kVecBytes - 1)) == 0;
     const T* base = src - s.head;
     T* out = dst - s.head;
-    const uint64_t policy = l2_policy(false);  // what the norm's pass kept is done with
+    const uint64_t policy = l2_policy(Evict::kFirst);  // what the norm's pass kept is done with
     if (s.whole() && vec) {
         Vec<T> x[kUnroll];
 #pragma unroll
@@ -172,7 +172,8 @@ int norm_of(int count, const void* const* grads, const long long* n, const unsig
         const unsigned int grid = std::min((t.chunks + kTeams - 1) / kTeams,
                                            static_cast<unsigned int>(std::min(kNormBlocks * sm_count(), kMaxPartials)));
         SPLAT_FOR_NORM(norm_type, NORM,
-                       (k_norm_partials<CAP, NORM><<<grid, kNormThreads, 0, st>>>(t, partials + used, keep ? kKeepChunks : 0u)));
+                       (k_norm_partials<CAP, NORM>
+                        <<<grid, kNormThreads, 0, st>>>(t, partials + used, keep ? kKeepChunks : 0u)));
         note_launch();
         used += static_cast<int>(grid);
         SPLAT_TRY(check_launch("gradient norm"));
@@ -317,9 +318,9 @@ int splat_grad_norm(int count, const void* const* grads, const long long* n, con
                     void* norm, int norm_is_f64, void* workspace, size_t workspace_bytes, void* stream) {
     SPLAT_TRY(gradnorm::check_list("splat_grad_norm", count, grads, n, dtypes, norm_is_f64));
     SPLAT_REQUIRE(gradnorm::known_norm(norm_type), "splat_grad_norm: unknown norm type %d", norm_type);
-    SPLAT_REQUIRE(norm, "splat_grad_norm: the norm's buffer is missing");
-    SPLAT_REQUIRE(workspace && workspace_bytes >= gradnorm::partial_bytes(count),
-                  "splat_grad_norm: workspace too small");
+    SPLAT_REQUIRE(gradnorm::aligned(norm, norm_is_f64), "splat_grad_norm: the norm's buffer is missing or not aligned");
+    SPLAT_REQUIRE(gradnorm::aligned(workspace, true) && workspace_bytes >= gradnorm::partial_bytes(count),
+                  "splat_grad_norm: workspace too small or not aligned");
     const gradnorm::Clip c{norm, 0.0, norm_is_f64};
     const cudaStream_t st = as_stream(stream);
     if (gradnorm::is_small(count, grads, n, dtypes))
@@ -334,10 +335,10 @@ int splat_grad_clip(int count, const void* const* grads, void* const* outs, cons
     SPLAT_REQUIRE(norm_type == SPLAT_NORM_GIVEN || gradnorm::known_norm(norm_type),
                   "splat_grad_clip: unknown norm type %d", norm_type);
     SPLAT_REQUIRE(max_norm >= 0.0, "splat_grad_clip: max_norm must not be negative");
-    SPLAT_REQUIRE(norm, "splat_grad_clip: the norm's buffer is missing");
+    SPLAT_REQUIRE(gradnorm::aligned(norm, norm_is_f64), "splat_grad_clip: the norm's buffer is missing or not aligned");
     const bool given = norm_type == SPLAT_NORM_GIVEN;
-    SPLAT_REQUIRE(given || (workspace && workspace_bytes >= gradnorm::partial_bytes(count)),
-                  "splat_grad_clip: workspace too small");
+    SPLAT_REQUIRE(given || (gradnorm::aligned(workspace, true) && workspace_bytes >= gradnorm::partial_bytes(count)),
+                  "splat_grad_clip: workspace too small or not aligned");
     SPLAT_REQUIRE(count == 0 || outs, "splat_grad_clip: the list of outputs is missing");
     int same = 0, other = 0;
     for (int i = 0; i < count; ++i) {

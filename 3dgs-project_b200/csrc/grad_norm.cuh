@@ -165,21 +165,26 @@ __device__ __forceinline__ void add(double& acc, double g) {
         acc = max_nan(acc, fabs(g));
 }
 
-// A 16-byte load with an L2 policy of l2_policy(): the line is evicted last (`keep`) or first.
+// How soon the L2 lets go of the lines that a load brings in.
+enum class Evict { kFirst, kNormal, kLast };
+
+__device__ __forceinline__ uint64_t l2_policy(Evict e) {
+    uint64_t p;
+    if (e == Evict::kLast)
+        asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    else if (e == Evict::kNormal)
+        asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    else
+        asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
 __device__ __forceinline__ uint4 load_hinted(const void* p, uint64_t policy) {
     uint4 v;
     asm volatile("ld.global.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p), "l"(policy));
     return v;
-}
-__device__ __forceinline__ uint64_t l2_policy(bool keep) {
-    uint64_t p;
-    if (keep)
-        asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
-    else
-        asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
-    return p;
 }
 
 template <typename T>
@@ -244,8 +249,8 @@ __device__ __forceinline__ void accumulate(const T* src, long long n, uint32_t c
     }
 }
 
-// This thread's share of the sum over chunks team, team + teams, ... of the table. The last `keep` chunks are kept in
-// the L2 for the pass that follows, the others leave it first.
+// This thread's share of the sum over chunks team, team + teams, ... of the table. With `keep`, the last so many chunks
+// are kept in the L2 for the pass that follows, and the others leave it first.
 template <int CAP, int NORM>
 __device__ __forceinline__ double accumulate_table(const Table<CAP>& t, uint32_t team, uint32_t teams, int thread,
                                                    uint32_t keep) {
@@ -254,7 +259,8 @@ __device__ __forceinline__ double accumulate_table(const Table<CAP>& t, uint32_t
         const int k = tensor_of(t, c);
         const uint32_t chunk = c - t.first_chunk[k];
         const void* src = t.src[k];
-        const uint64_t policy = l2_policy(t.chunks - c <= keep);
+        const uint64_t policy =
+            l2_policy(keep == 0 ? Evict::kNormal : t.chunks - c <= keep ? Evict::kLast : Evict::kFirst);
         switch (t.dtype[k]) {
             case SPLAT_F32:
                 accumulate<float, NORM>(static_cast<const float*>(src), t.n[k], chunk, thread, policy, acc);
@@ -299,7 +305,7 @@ __device__ __forceinline__ double cluster_norm(const Table<CAP>& t, int norm_f64
     constexpr int kTeams = kSmallThreads / kTeam;
     const uint32_t rank = cluster.block_rank();
     double acc = accumulate_table<CAP, NORM>(t, rank * kTeams + threadIdx.x / kTeam, kSmallCluster * kTeams,
-                                             threadIdx.x % kTeam, kSmallChunks);
+                                             threadIdx.x % kTeam, 0u);
     acc = block_total<kSmallThreads, NORM>(acc);
     if (threadIdx.x == 0) s_block = acc;
     cluster.sync();
@@ -320,6 +326,9 @@ inline bool known_norm(int norm_type) {
 }
 
 inline int size_of(int dtype) { return dtype == SPLAT_F32 ? 4 : dtype == SPLAT_F64 ? 8 : 2; }
+
+// A buffer of float32 or float64 values that is there.
+inline bool aligned(const void* p, bool f64) { return p && reinterpret_cast<uintptr_t>(p) % (f64 ? 8 : 4) == 0; }
 
 inline long long chunks_of(const void* src, long long n, int dtype) {
     const uintptr_t head = reinterpret_cast<uintptr_t>(src) & (kVecBytes - 1);

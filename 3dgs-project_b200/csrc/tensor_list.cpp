@@ -76,6 +76,14 @@ PyObject* describe(PyObject*, PyObject* seq) {
     }
 }
 
+// Two tensors of one shape lie alike in memory: their strides agree where a dimension has more than one entry.
+bool lie_alike(const at::Tensor& x, const at::Tensor& y) {
+    if (x.numel() == 0 || (x.is_contiguous() && y.is_contiguous())) return true;
+    for (int64_t d = 0; d < x.dim(); ++d)
+        if (x.size(d) != 1 && x.stride(d) != y.stride(d)) return false;
+    return true;
+}
+
 // same_form(a, b) -> whether the two lists' tensors agree one by one in shape, type and (with elements) strides.
 PyObject* same_form(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != 2) {
@@ -89,8 +97,7 @@ PyObject* same_form(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (!THPVariable_Check(a.items[i]) || !THPVariable_Check(b.items[i])) Py_RETURN_FALSE;
             const at::Tensor &x = THPVariable_Unpack(a.items[i]), &y = THPVariable_Unpack(b.items[i]);
             if (x.scalar_type() != y.scalar_type() || x.sizes() != y.sizes()) Py_RETURN_FALSE;
-            if (x.numel() > 0 && !(x.is_contiguous() && y.is_contiguous()) && x.strides() != y.strides())
-                Py_RETURN_FALSE;
+            if (!lie_alike(x, y)) Py_RETURN_FALSE;
         }
     } catch (const std::exception&) {
         Py_RETURN_FALSE;

@@ -394,7 +394,7 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
  * null pointers.
  * The arrays are read during the call only. *norm is device memory: float32, or float64 when norm_is_f64, which a list
  * with a float64 tensor needs.
- * workspace: device scratch of splat_grad_workspace_size(count) bytes, not kept between calls; calls that may run at
+ * workspace: device scratch of splat_grad_workspace_size(count) bytes, 8-byte aligned, not kept between calls; calls that may run at
  * the same time (other streams, graphs replayed side by side) need one each.
  * ------------------------------------------------------------------------------------------- */
 #define SPLAT_F32 0

@@ -51,7 +51,10 @@ def _error() -> str:
     (dict(norm_type=3), "unknown norm type"),
     (dict(norm_type=-1), "unknown norm type"),
     (dict(norm=None), "norm's buffer"),
+    (dict(norm=P + 2), "norm's buffer"),
+    (dict(norm=P + 4, f64=1), "norm's buffer"),
     (dict(ws=None), "workspace"),
+    (dict(ws=P + 4), "workspace"),
     (dict(ws_bytes=8), "workspace"),
 ])
 def test_norm_refusals(kw, says):
@@ -94,8 +97,8 @@ def test_many_tensors_that_overlap_are_found():
 
 
 @pytest.mark.parametrize("kw,says", [(dict(norm_type=9), "norm type"), (dict(max_norm=-0.5), "max_norm"),
-                                     (dict(norm=None), "norm's buffer"), (dict(ws=None), "workspace"),
-                                     (dict(step=0), "step"), (dict(n=-1), "size")])
+                                     (dict(norm=None), "norm's buffer"), (dict(norm=P + 1), "norm's buffer"),
+                                     (dict(ws=None), "workspace"), (dict(ws=P + 1), "workspace"), (dict(step=0), "step"), (dict(n=-1), "size")])
 @pytest.mark.parametrize("lean", [False, True])
 def test_clipped_step_refusals(lean, kw, says):
     a = dict(step=1, norm_type=2, max_norm=1.0, norm=P, ws=P, n=4)
@@ -174,6 +177,19 @@ def test_nothing_to_do():
 def test_fuse_backward_is_refused():
     with pytest.raises(RuntimeError, match="fuse_backward"):
         A.FusedAdam([torch.nn.Parameter(torch.zeros(3))], lr=1e-3, eps=1e-15, fuse_backward=True, max_grad_norm=1.0)
+
+
+def test_forms_that_agree():
+    same = G._tensors().same_form
+    x = torch.zeros(4, 5, 6)
+    assert same([x], [torch.zeros(4, 5, 6)]) and same([], [])
+    assert not same([x], [torch.zeros(4, 5, 7)]) and not same([x], [x.double()]) and not same([x], [x, x])
+    assert not same([x.transpose(0, 1)], [torch.zeros(5, 4, 6)])
+    assert same([x.transpose(0, 1)], [torch.ones(4, 5, 6).transpose(0, 1)])
+    # the stride of a dimension with one entry says nothing
+    a = torch.zeros(9, 1, 2).as_strided((2, 1, 9), (1, 7, 2))
+    assert same([a], [torch.zeros(9, 1, 2).as_strided((2, 1, 9), (1, 2, 2))])
+    assert not same([x], ["x"])
 
 
 def test_dense_orders():

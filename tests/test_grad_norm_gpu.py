@@ -8,10 +8,14 @@ subnormal where the product is that small."""
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
+from gs_b200 import _lib as L
 from gs_b200 import adam as A
 from gs_b200 import grad as G
 from gs_b200 import gs3d, scenes
@@ -547,6 +551,47 @@ def test_sparse_optimizer(cuda):
             oa.zero_grad()
     finally:
         gs3d._Rasterize.track_visibility = False
+
+
+def test_kernel_timer(cuda):
+    """The timer's events between the launches of a clipped step change nothing."""
+    for n in (100, 60_000):
+        a = adam_state(n, cuda, 8)
+        b = copies(a)
+        want = A.adam_step(a, 3, max_grad_norm=0.1)
+        with L.KernelTimer("k_adam") as timer:
+            timer.arm()
+            got = A.adam_step(b, 3, max_grad_norm=0.1)
+        assert len(timer.times()["k_adam"]) == 1 and timer.times()["k_adam"][0] > 0
+        assert torch.equal(got, want)
+        same_groups(a, b)
+
+
+def test_first_call_inside_a_capture(cuda):
+    """In a process of its own whose first call of each entry point is captured."""
+    code = """
+import torch
+from __graft_entry__ import load_package
+load_package()
+from gs_b200 import adam as A, grad as G
+g = [torch.ones(70_000, 3, device="cuda"), torch.ones(7, device="cuda")]
+one = [torch.ones(5, device="cuda")]
+p, m, v = ([torch.ones_like(t) for t in g] for _ in range(3))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    norms = [G.grad_norm(g), G.grad_norm(one)]
+    outs = G.clip_grads(g, 1.0)[0] + G.clip_grads(one, 1.0)[0]
+    norms.append(A.adam_step(list(zip(p, g, m, v, (1e-3, 1e-3))), 1, max_grad_norm=1.0))
+graph.replay()
+torch.cuda.synchronize()
+n = 210_007 ** 0.5
+assert abs(float(norms[0]) - n) < 1e-3 and abs(float(norms[1]) - 5 ** 0.5) < 1e-6 and float(norms[2]) == float(norms[0])
+assert abs(float(outs[0][0, 0]) - 1 / n) < 1e-8 and abs(float(outs[2][0]) - 5 ** -0.5) < 1e-6
+assert float(p[1][0]) < 1.0
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_calls_for_another_device_than_the_current_one(cuda):
