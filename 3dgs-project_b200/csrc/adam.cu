@@ -111,8 +111,7 @@ __global__ void __launch_bounds__(kThreads, 5)
     k_adam_clipped(const __grid_constant__ Table t, const __grid_constant__ gradnorm::Clip c) {
     const long long tile = gridDim.x - 1u - blockIdx.x;
     const Group& G = t.g[group_of(t, tile)];
-    gradnorm::wait_for_primary();
-    const float f = static_cast<float>(gradnorm::factor_of(gradnorm::load_norm(c), c.max_norm));
+    const float f = static_cast<float>(gradnorm::block_factor(c));
     adam_tile<true>(G, t, (tile - G.first_block) * kPerBlock, threadIdx.x, f);
 }
 
@@ -393,8 +392,7 @@ template <bool kMasked>
 __global__ void __launch_bounds__(kThreads, kMasked ? 6 : 1)
     k_adam_lean_clipped(const __grid_constant__ LeanTable t, const __grid_constant__ gradnorm::Clip c) {
     __shared__ uint16_t s_list[kThreads / 32][kLeanList];
-    gradnorm::wait_for_primary();
-    const float f = static_cast<float>(gradnorm::factor_of(gradnorm::load_norm(c), c.max_norm));
+    const float f = static_cast<float>(gradnorm::block_factor(c));
     lean_tile<true, kMasked>(t, gridDim.x - 1u - blockIdx.x, threadIdx.x, s_list[threadIdx.x / 32], f);
 }
 
@@ -528,7 +526,7 @@ int clipped_step(const char* what, int count, const G* groups, const T& table, l
                      : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,
                                        stream);
     const cudaStream_t st = as_stream(stream);
-    const gradnorm::Clip c{norm, max_norm, 0};
+    gradnorm::Clip c{norm, max_norm, 0};
     if (!given) {
         Grads list{};  // dtype 0: SPLAT_F32
         for (int i = 0; i < count; ++i) {
@@ -553,7 +551,7 @@ int clipped_step(const char* what, int count, const G* groups, const T& table, l
             return check_launch(what);
         }
         SPLAT_TRY(gradnorm::enqueue_norm(count, list.grad, list.n, list.dtype, norm_type,
-                                         static_cast<double*>(workspace), c, true, st));
+                                         static_cast<double*>(workspace), c, gradnorm::Again::kAll, st));
     }
     cudaError_t e = cudaSuccess;
     SPLAT_TIMED_LAUNCH("k_adam", st,

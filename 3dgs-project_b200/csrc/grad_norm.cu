@@ -31,6 +31,11 @@ constexpr int kNormBlocks = 4;  // per SM: all its threads
 // What the norm's pass keeps in the L2 for a second one: 64 MiB of its 126 MB (32 MiB: 110.0 us for the 1M Gaussians
 // above, 96 MiB: 108.5, 64 MiB: 107.5).
 constexpr uint32_t kKeepChunks = 4096;
+// Lists of up to 2048 chunks (32 MiB) leave the partials to the blocks that scale or step, each of which reduces them
+// for itself: one launch less, 3 us of the host's time, and on the device 6.5 against 7.4 us for clipping 20 thousand
+// 3D Gaussians' gradients and 31.9 against 32.6 for the step of 100 thousand. Longer lists have too many blocks for
+// that: the lean step of 1M Gaussians takes 214 us so and 207 after k_norm_finish.
+constexpr long long kDirectChunks = 2048;
 constexpr int kScaleThreads = kTeam;
 // Out of place a block scales one chunk: a resident grid that loops took 84 us where this takes 72 (1M Gaussians, 236 MB
 // read and written). In place most calls find a factor of 1 and end there, and blocks that only end cost time too: with
@@ -60,8 +65,7 @@ __global__ void __launch_bounds__(kNormThreads)
     if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
-// One warp reduces the partials. Doing so at the start of every block that scales saves this launch (1 us with 100k Gaussians), but needs a
-// resident grid, which scales and steps more slowly (see k_clip_scale's and k_adam_clipped's figures).
+// One warp reduces the partials, for a norm alone or a long list.
 __global__ void __launch_bounds__(32) k_norm_finish(const double* partials, int count, int norm_type, Clip c) {
     release_dependents();
     wait_for_primary();
@@ -141,8 +145,7 @@ __device__ __forceinline__ void scale_table(const Table<CAP>& t, uint32_t team, 
 template <int CAP>
 __global__ void __launch_bounds__(kScaleThreads)
     k_clip_scale(const __grid_constant__ Table<CAP> t, const __grid_constant__ Clip c, int in_place) {
-    wait_for_primary();
-    const double f = factor_of(load_norm(c), c.max_norm);
+    const double f = block_factor(c);
     if (in_place && f == 1.0) return;  // x * 1 is x, NaN and infinities too
     scale_table(t, blockIdx.x, gridDim.x, threadIdx.x, f);
 }
@@ -162,9 +165,10 @@ __global__ void __launch_bounds__(kSmallThreads)
 
 template <int CAP>
 int norm_of(int count, const void* const* grads, const long long* n, const unsigned char* dtypes, int norm_type,
-            double* partials, const Clip& c, bool keep, cudaStream_t st) {
+            double* partials, Clip& c, Again again, cudaStream_t st) {
     Table<CAP> t;
     int used = 0;
+    long long chunks = 0;
     for (int i = 0; i < count;) {
         i = fill(t, i, count, grads, nullptr, n, dtypes);
         if (t.count == 0) break;
@@ -173,10 +177,17 @@ int norm_of(int count, const void* const* grads, const long long* n, const unsig
                                            static_cast<unsigned int>(std::min(kNormBlocks * sm_count(), kMaxPartials)));
         SPLAT_FOR_NORM(norm_type, NORM,
                        (k_norm_partials<CAP, NORM>
-                        <<<grid, kNormThreads, 0, st>>>(t, partials + used, keep ? kKeepChunks : 0u)));
+                        <<<grid, kNormThreads, 0, st>>>(t, partials + used, again == Again::kAll ? kKeepChunks : 0u)));
         note_launch();
         used += static_cast<int>(grid);
+        chunks += t.chunks;
         SPLAT_TRY(check_launch("gradient norm"));
+    }
+    if (again != Again::kNo && chunks <= kDirectChunks) {
+        c.partials = partials;
+        c.count = used;
+        c.norm_type = norm_type;
+        return SPLAT_OK;
     }
     SPLAT_CUDA(launch(k_norm_finish, 1, 32, st, used > 0, 1, static_cast<const double*>(partials), used, norm_type, c));
     note_launch();
@@ -203,8 +214,8 @@ int norm_of(int count, const void* const* grads, const long long* n, const unsig
     } while (0)
 
 int enqueue_norm(int count, const void* const* grads, const long long* n, const unsigned char* dtypes, int norm_type,
-                 double* partials, const Clip& c, bool keep, cudaStream_t st) {
-    SPLAT_FOR_TABLE(count, CAP, return norm_of<CAP>(count, grads, n, dtypes, norm_type, partials, c, keep, st));
+                 double* partials, Clip& c, Again again, cudaStream_t st) {
+    SPLAT_FOR_TABLE(count, CAP, return norm_of<CAP>(count, grads, n, dtypes, norm_type, partials, c, again, st));
 }
 
 // One launch for a list that fits one small table.
@@ -321,11 +332,12 @@ int splat_grad_norm(int count, const void* const* grads, const long long* n, con
     SPLAT_REQUIRE(gradnorm::aligned(norm, norm_is_f64), "splat_grad_norm: the norm's buffer is missing or not aligned");
     SPLAT_REQUIRE(gradnorm::aligned(workspace, true) && workspace_bytes >= gradnorm::partial_bytes(count),
                   "splat_grad_norm: workspace too small or not aligned");
-    const gradnorm::Clip c{norm, 0.0, norm_is_f64};
+    gradnorm::Clip c{norm, 0.0, norm_is_f64};
     const cudaStream_t st = as_stream(stream);
     if (gradnorm::is_small(count, grads, n, dtypes))
         return gradnorm::run_small(count, grads, nullptr, n, dtypes, norm_type, c, 0, st);
-    return gradnorm::enqueue_norm(count, grads, n, dtypes, norm_type, static_cast<double*>(workspace), c, false, st);
+    return gradnorm::enqueue_norm(count, grads, n, dtypes, norm_type, static_cast<double*>(workspace), c,
+                                  gradnorm::Again::kNo, st);
 }
 
 int splat_grad_clip(int count, const void* const* grads, void* const* outs, const long long* n,
@@ -349,7 +361,7 @@ int splat_grad_clip(int count, const void* const* grads, void* const* outs, cons
         ++(outs[i] == grads[i] ? same : other);
     }
     SPLAT_REQUIRE(same == 0 || other == 0, "splat_grad_clip: some tensors are clipped in place, others are not");
-    const gradnorm::Clip c{norm, max_norm, norm_is_f64};
+    gradnorm::Clip c{norm, max_norm, norm_is_f64};
     SPLAT_TRY(gradnorm::check_overlap(count, grads, outs, n, dtypes, same > 0, c, given));
     const cudaStream_t st = as_stream(stream);
     if (!given) {
@@ -358,7 +370,7 @@ int splat_grad_clip(int count, const void* const* grads, void* const* outs, cons
         if (gradnorm::is_small(count, grads, n, dtypes))
             return gradnorm::run_small(count, grads, outs, n, dtypes, norm_type, c, same > 0, st);
         SPLAT_TRY(gradnorm::enqueue_norm(count, grads, n, dtypes, norm_type, static_cast<double*>(workspace), c,
-                                         same == 0, st));
+                                         same ? gradnorm::Again::kInPlace : gradnorm::Again::kAll, st));
     }
     return gradnorm::enqueue_scaling(count, grads, outs, n, dtypes, c, same > 0, !given, st);
 }

@@ -3,8 +3,9 @@
 // bits as the step that clips.
 //
 // The norm of a long list is taken in two stages: each block of the norm kernel leaves one float64 partial (a sum of
-// squares, a sum of absolute values, or a maximum) in the workspace, and one warp reduces the few hundred of them, so no
-// atomic decides an order. A short list takes one launch, in which the blocks of a cluster exchange their partials.
+// squares, a sum of absolute values, or a maximum) in the workspace, and one warp, of a kernel of its own or of every
+// block that uses the norm, reduces the few hundred of them in an order that depends on their number only. A short list
+// takes one launch, in which the blocks of a cluster exchange their partials.
 //   norm = sqrt(sum), sum or max, rounded once to the caller's type (float32, or float64)
 //   factor = min(1, max_norm / (norm + 1e-6)) in float64 from the rounded norm; NaN where the norm is NaN
 #pragma once
@@ -29,8 +30,8 @@ constexpr int kMaxPartials = 1024;  // of one launch
 // Lists of at most kSmallChunks chunks (1 MiB) take one launch: a cluster reads them all and adds its blocks' sums
 // through distributed shared memory. Eight SMs are slower than all of them on the longer of these lists, but each launch
 // saved is 3 us of the host's time. The norm of 43 chunks (3000 3D Gaussians): 5.0 us on the device and 9.8 us a call,
-// against 3.5 and 12.7 in two launches. At 86 chunks clipping takes 12.3 us on the device and 16.0 a call, against 6.3
-// and 17.4 in three: there the device has caught up with the host.
+// against 3.5 and 12.7 in two launches. At 86 chunks clipping takes 12.3 us on the device and 16.0 a call, against 5.6
+// and 15.7 in two: there the device has caught up with the host.
 constexpr int kSmallCluster = 8;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallChunks = 64;
@@ -51,11 +52,15 @@ struct Table {
     uint32_t chunks;
 };
 
-// Where the clip factor comes from: a norm in device memory, the caller's or one that the launch before computed.
+// Where the clip factor comes from: a norm in device memory, the caller's or one that the launch before computed, or
+// (partials given) the partials of the launch before, which every block reduces for itself and block 0 stores as *norm.
 struct Clip {
     void* norm;
     double max_norm;
     int norm_f64;  // *norm is float64
+    int norm_type;
+    int count;
+    const double* partials;
 };
 
 // ---- programmatic dependent launch: the second kernel of a call starts while the first one drains ----
@@ -133,6 +138,22 @@ __device__ __forceinline__ double factor_of(double norm, double max_norm) {
 
 __device__ __forceinline__ double load_norm(const Clip& c) {
     return c.norm_f64 ? *static_cast<const double*>(c.norm) : static_cast<double>(*static_cast<const float*>(c.norm));
+}
+
+// The clip factor, in every thread of the block (which must call it as one), once the launch before has finished.
+__device__ __forceinline__ double block_factor(const Clip& c) {
+    __shared__ double s_factor;
+    wait_for_primary();
+    if (!c.partials) return factor_of(load_norm(c), c.max_norm);
+    if (threadIdx.x < 32) {
+        const double norm = rounded_norm(warp_total(c.partials, c.count, c.norm_type), c.norm_type, c.norm_f64);
+        if (threadIdx.x == 0) {
+            if (blockIdx.x == 0) store_norm(c, norm);
+            s_factor = factor_of(norm, c.max_norm);
+        }
+    }
+    __syncthreads();
+    return s_factor;
 }
 
 // The tensor that a chunk belongs to: the last one whose first chunk is not behind it (empty tensors are not in the
@@ -381,10 +402,13 @@ inline bool is_small(int count, const void* const* grads, const long long* n, co
     return chunks <= kSmallChunks;
 }
 
+enum class Again { kNo, kInPlace, kAll };
+
 // The norm of a list that is not small, stored as `c` says (grad_norm.cu). Arguments already checked. The kernel that
-// uses it can be launched as a dependent. keep: it reads all of the list again, and is to find the end in the L2.
+// uses it can be launched as a dependent. again: it reads all of the list again, is to find the end in the L2, and takes
+// its factor with block_factor(), for which a list of middling length leaves the partials in `c`.
 int enqueue_norm(int count, const void* const* grads, const long long* n, const unsigned char* dtypes, int norm_type,
-                 double* partials, const Clip& c, bool keep, cudaStream_t stream);
+                 double* partials, Clip& c, Again again, cudaStream_t stream);
 
 }  // namespace gradnorm
 }  // namespace splat
