@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/ops/empty.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -115,18 +116,15 @@ PyObject* scratch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int f64 = PyObject_IsTrue(args[1]);
     const long long bytes = PyLong_AsLongLong(args[2]);
     if (PyErr_Occurred()) return nullptr;
-    try {
-        const auto on = at::TensorOptions().device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
-        at::Tensor norm = at::empty({}, on.dtype(f64 ? at::kDouble : at::kFloat));
-        at::Tensor space = at::empty({bytes}, on.dtype(at::kByte));
-        const auto norm_at = reinterpret_cast<unsigned long long>(norm.data_ptr());
-        const auto space_at = reinterpret_cast<unsigned long long>(space.data_ptr());
-        return Py_BuildValue("(NKNK)", THPVariable_Wrap(std::move(norm)), norm_at, THPVariable_Wrap(std::move(space)),
-                             space_at);
-    } catch (const std::exception& e) {  // out of memory
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
-    }
+    HANDLE_TH_ERRORS  // out of memory is torch.OutOfMemoryError
+    const auto on = at::TensorOptions().device(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+    at::Tensor norm = at::empty({}, on.dtype(f64 ? at::kDouble : at::kFloat));
+    at::Tensor space = at::empty({bytes}, on.dtype(at::kByte));
+    const auto norm_at = reinterpret_cast<unsigned long long>(norm.data_ptr());
+    const auto space_at = reinterpret_cast<unsigned long long>(space.data_ptr());
+    return Py_BuildValue("(NKNK)", THPVariable_Wrap(std::move(norm)), norm_at, THPVariable_Wrap(std::move(space)),
+                         space_at);
+    END_HANDLE_TH_ERRORS
 }
 
 // adam_table(groups, lean) -> (adam_group or adam_lean_group array as bytes, device index, whether that is the current

@@ -9,7 +9,7 @@ The Adam steps of gs_b200.adam take max_grad_norm and clip as they read the grad
 Tensors are float32, bfloat16, float16 or float64 CUDA tensors, mixed in one call, each dense in its own order of
 dimensions (contiguous, transposed, channels-last), of any length and at any address. Sums are taken in float64 in an
 order that the sizes fix, so a call repeats bit for bit. None of the calls waits for the device (error_if_nonfinite
-apart), and all can be captured into a CUDA graph.
+apart), and all can be captured into a CUDA graph. Nothing is recorded for autograd.
 """
 from __future__ import annotations
 

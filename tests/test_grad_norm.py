@@ -179,6 +179,13 @@ def test_fuse_backward_is_refused():
         A.FusedAdam([torch.nn.Parameter(torch.zeros(3))], lr=1e-3, eps=1e-15, fuse_backward=True, max_grad_norm=1.0)
 
 
+def test_buffers_that_cannot_be_had():
+    with pytest.raises(RuntimeError):
+        G._tensors().scratch(0, False, 1 << 62)  # no such memory; without a GPU, no CUDA either
+    with pytest.raises(TypeError):
+        G._tensors().scratch(0, False)
+
+
 def test_forms_that_agree():
     same = G._tensors().same_form
     x = torch.zeros(4, 5, 6)
