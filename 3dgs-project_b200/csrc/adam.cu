@@ -172,8 +172,10 @@ __device__ __forceinline__ uint32_t lowbias32(uint32_t x) {
 
 __device__ __forceinline__ float bf16_to_float(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
 
-// Stochastic rounding to bfloat16: uniform noise in the 16 bits that are dropped, then truncation.
+// Stochastic rounding to bfloat16: uniform noise in the 16 bits that are dropped, then truncation. NaN stays NaN: noise
+// added to its bits would carry through the exponent into the sign and leave -0 or 0.
 __device__ __forceinline__ uint16_t float_to_bf16_sr(float f, uint32_t rnd) {
+    if (f != f) return 0x7FFFu;
     return static_cast<uint16_t>((__float_as_uint(f) + (rnd & 0xFFFFu)) >> 16);
 }
 

@@ -4,7 +4,8 @@ Follows `adam_step_sparse_cu<LOWP>` of cluster/patches/fastergs_lean_adam.patch:
   hash_u32 (:72-75)      the lowbias32 integer hash (C. Wellons), two multiply-xorshift rounds
   bf16 read (:77-79)     bits << 16
   SR write (:83-86)      (bits(f) + (rnd & 0xFFFF)) >> 16, rnd = hash((uint32) i ^ seed) for exp_avg and
-                         hash of that for exp_avg_sq (:122-123), seed = 0x9E3779B9 * step + 0x85EBCA6B (:165)
+                         hash of that for exp_avg_sq (:122-123), seed = 0x9E3779B9 * step + 0x85EBCA6B (:165);
+                         NaN is kept, as the bits 0x7FFF (the patch's sum carries it into the sign: -0)
   update (:116-120)      m = fma(b1, m - g, g); v = fma(b2, v - g^2, g^2); p -= step_size * m / fma(sqrt(v), bc2, eps)
   mask (:106)            element i is skipped when visibility[i // features] == 0
 numpy uint32 arithmetic wraps like the device's. The update below uses float64 for the fused multiply-adds, which
@@ -37,8 +38,9 @@ def bf16_bits_to_float(bits) -> np.ndarray:
 
 
 def float_to_bf16_bits_sr(f, rnd) -> np.ndarray:
-    u = np.asarray(f, dtype=np.float32).view(U32)
-    return ((u + (np.asarray(rnd, dtype=U32) & U32(0xFFFF))) >> U32(16)).astype(np.uint16)
+    f = np.asarray(f, dtype=np.float32)
+    rounded = ((f.view(U32) + (np.asarray(rnd, dtype=U32) & U32(0xFFFF))) >> U32(16)).astype(np.uint16)
+    return np.where(np.isnan(f), np.uint16(0x7FFF), rounded)
 
 
 def sr_randoms(n: int, step: int) -> tuple[np.ndarray, np.ndarray]:

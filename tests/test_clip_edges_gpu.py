@@ -1,0 +1,69 @@
+"""Edges of the gradient norm, the clipping and the clipped Adam steps on the GPU."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from gs_b200 import adam as A
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+SHAPES_3DGS = [(3,), (3,), (4,), (1,), (1, 3), (15, 3)]
+
+
+def adam_state(n, device, seed, lowp=(), offset=0):
+    """Groups of the six tensors of n 3D Gaussians, each `offset` elements behind the start of its allocation; moments
+    of the groups in `lowp` in bfloat16."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+
+    def make(shape, scale, dtype=F32):
+        flat = torch.empty(math.prod(shape) + offset, device=device, dtype=dtype)
+        return flat[offset:].view(shape).copy_(torch.randn(shape, generator=gen, device=device) * scale)
+
+    groups = []
+    for k, s in enumerate(SHAPES_3DGS):
+        dtype = BF16 if k in lowp else F32
+        p, g = make((n, *s), 1.0), make((n, *s), 10.0 ** -k)
+        groups.append((p, g, make((n, *s), 1e-2, dtype), make((n, *s), 1e-2, dtype).abs_(), 1e-3 * (k + 1)))
+    return groups
+
+
+def copies(groups):
+    return [(p.clone(), g.clone(), m.clone(), v.clone(), lr) for p, g, m, v, lr in groups]
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("n", [1, 7, 301, 4096, 30_011])
+def test_nan_in_bfloat16_moments(cuda, n, masked):
+    """One NaN gradient makes the clip factor NaN: every element that is updated gets NaN moments, in bfloat16 as in
+    float32, on vectors, their scalar ends and misaligned buffers, in one launch and in several. The elements that the
+    mask leaves out keep what they had."""
+    vis = None
+    if masked:
+        vis = (torch.rand(n, device=cuda, generator=torch.Generator(device=cuda).manual_seed(n)) < 0.5).int()
+        vis[0] = 1
+    for offset in (0, 1):
+        a = adam_state(n, cuda, n, lowp=(1, 5), offset=offset)
+        a[3][1][n // 2] = math.nan
+        b = copies(a)
+        assert math.isnan(float(A.adam_step_lean(a, 12, vis, max_grad_norm=1.0)))
+        for x, y in zip(a, b):
+            on = torch.ones(n, dtype=torch.bool, device=cuda) if vis is None else vis != 0
+            for i in (0, 2, 3):
+                assert bool(x[i][on].isnan().all()), (offset, x[0].shape, i)
+                assert torch.equal(x[i][~on], y[i][~on])
+
+
+def test_nan_in_bfloat16_moments_without_the_clip(cuda):
+    """The same of the step that does not clip: NaN where the gradient is, nowhere else."""
+    a = adam_state(5003, cuda, 3, lowp=(0, 1, 2, 3, 4, 5))
+    at = torch.randint(0, 5003, (97,), device=cuda)
+    for _, g, _, _, _ in a:
+        g[at] = math.nan
+    A.adam_step_lean(a, 5)
+    for p, g, m, v, _ in a:
+        for t in (p, m, v):
+            assert torch.equal(t.isnan(), g.isnan())
