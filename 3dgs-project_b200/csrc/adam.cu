@@ -475,8 +475,8 @@ int build_lean_table(const char* what, int count, const adam_lean_group* groups,
     int k = 0;
     for (int i = 0; i < count; ++i) {
         const adam_lean_group& g = groups[i];
-        SPLAT_REQUIRE(g.n >= 0 && g.features >= 1, "%s: group %d has a bad size", what, i);
-        if (g.n == 0) continue;
+        SPLAT_REQUIRE(g.n >= 0 && (g.n == 0 || g.features >= 1), "%s: group %d has a bad size", what, i);
+        if (g.n == 0) continue;  // rows of no elements (features 0) or no rows
         SPLAT_REQUIRE(g.param && g.grad && g.exp_avg && g.exp_avg_sq, "%s: group %d has a null buffer", what, i);
         SPLAT_REQUIRE(!visibility || g.n == static_cast<long long>(g.features) * n_primitives,
                       "%s: group %d has %lld elements, not %d x %lld primitives", what, i, g.n, g.features,

@@ -1,9 +1,17 @@
 """Edges of the gradient norm, the clipping and the clipped Adam steps that need no GPU."""
 from __future__ import annotations
 
-import numpy as np
+import ctypes
 
+import numpy as np
+import pytest
+
+from gs_b200 import _lib as L
+from gs_b200 import adam as A
 from oracle import adam_oracle as O
+
+OK, ERR_ARG = 0, 1
+P = 1 << 20  # an address that is never read: the calls below are refused, or have nothing to do
 
 
 def test_rounding_keeps_what_is_not_finite():
@@ -15,3 +23,20 @@ def test_rounding_keeps_what_is_not_finite():
     for sign in (1.0, -1.0):
         f = np.full(noise.size, sign * np.inf, np.float32)
         assert (O.bf16_bits_to_float(O.float_to_bf16_bits_sr(f, noise)) == sign * np.inf).all()
+
+
+def _lean_step(groups, visibility=None, n_primitives=0):
+    arr = (A._LeanGroup * len(groups))(*groups)
+    return L.load().adam_step_multi_lean(len(groups), ctypes.addressof(arr), 1, 0.9, 0.999, 1e-15, visibility,
+                                         n_primitives, None)
+
+
+@pytest.mark.parametrize("features", [0, 1, 45])
+def test_lean_groups_without_elements(features):
+    """Rows of no elements, or no rows: nothing to do. A group with elements has rows of at least one."""
+    empty = A._LeanGroup(None, None, None, None, 0, 1e-3, features, 1)
+    assert _lean_step([empty, empty]) == OK
+    assert _lean_step([empty], P, 0) == OK
+    assert _lean_step([empty, A._LeanGroup(P, P, P, P, 4, 1e-3, 0, 0)]) == ERR_ARG
+    assert "bad size" in L.load().splat_last_error().decode()
+    assert _lean_step([A._LeanGroup(P, P, P, P, -4, 1e-3, 1, 0)]) == ERR_ARG

@@ -67,3 +67,28 @@ def test_nan_in_bfloat16_moments_without_the_clip(cuda):
     for p, g, m, v, _ in a:
         for t in (p, m, v):
             assert torch.equal(t.isnan(), g.isnan())
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("clip", [{}, {"max_grad_norm": 0.05}])
+def test_lean_groups_without_elements(cuda, clip, masked):
+    """A model of SH degree 0 has no higher bases (n, 0, 3): the lean steps pass over that group."""
+    n = 501
+    vis = (torch.rand(n, device=cuda) < 0.4).int() if masked else None
+    a = adam_state(n, cuda, 6, lowp=(4,))
+    b = copies(a)
+    none = torch.empty(n, 0, 3, device=cuda)
+    low = none.bfloat16()
+    total = A.adam_step_lean(a[:2] + [(none, none, low, low, 1e-3)] + a[2:], 4, vis, **clip)
+    want = A.adam_step_lean(b, 4, vis, **clip)
+    assert total is None if want is None else torch.equal(total, want)
+    for x, y in zip(a, b):
+        assert all(torch.equal(x[i], y[i]) for i in (0, 1, 2, 3))
+    for rows in (0, n):  # nothing at all
+        t = torch.empty(rows, 0, 3, device=cuda)
+        seen = torch.zeros(rows, dtype=torch.int32, device=cuda) if masked else None
+        total = A.adam_step_lean([(t, t, t, t, 1e-3)], 4, seen, **clip)
+        assert total is None if not clip else float(total) == 0.0
+    t = torch.empty(0, 3, device=cuda)  # no Gaussians
+    total = A.adam_step_lean([(t, t, t, t, 1e-3)], 4, vis[:0] if masked else None, **clip)
+    assert total is None if not clip else float(total) == 0.0
