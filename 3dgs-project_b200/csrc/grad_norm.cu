@@ -266,16 +266,20 @@ int check_list(const char* what, int count, const void* const* grads, const long
                const unsigned char* dtypes, int norm_f64) {
     SPLAT_REQUIRE(count >= 0, "%s: negative count", what);
     SPLAT_REQUIRE(count == 0 || (grads && n && dtypes), "%s: the list of tensors is missing", what);
+    long long chunks = 0;
     for (int i = 0; i < count; ++i) {
         SPLAT_REQUIRE(n[i] >= 0, "%s: tensor %d has negative size", what, i);
         SPLAT_REQUIRE(dtypes[i] <= SPLAT_F64, "%s: tensor %d has an unknown type", what, i);
-        // 32 TiB; chunk counts stay in 32 bits
-        SPLAT_REQUIRE(n[i] <= (1ll << 45) / size_of(dtypes[i]), "%s: tensor %d has %lld elements", what, i, n[i]);
+        SPLAT_REQUIRE(n[i] <= (1ll << 45) / size_of(dtypes[i]), "%s: tensor %d has %lld elements", what, i, n[i]);  // 32 TiB
         SPLAT_REQUIRE(dtypes[i] != SPLAT_F64 || norm_f64, "%s: tensor %d is float64, the norm is not", what, i);
         if (n[i] == 0) continue;
         SPLAT_REQUIRE(grads[i], "%s: tensor %d has a null buffer", what, i);
         SPLAT_REQUIRE(reinterpret_cast<uintptr_t>(grads[i]) % size_of(dtypes[i]) == 0,
                       "%s: tensor %d is not aligned to its type", what, i);
+        chunks += chunks_of(grads[i], n[i], dtypes[i]);
+        // No device holds as much, but a list may name a tensor many times. A kernel's chunk index, raised by less than
+        // 2^31 at a time, stays in 32 bits so, and every launch has its place in the workspace.
+        SPLAT_REQUIRE(chunks < (1ll << 31), "%s: the tensors have more than 32 TiB together", what);
     }
     return SPLAT_OK;
 }

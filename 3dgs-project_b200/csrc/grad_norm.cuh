@@ -356,7 +356,8 @@ inline long long chunks_of(const void* src, long long n, int dtype) {
     return (static_cast<long long>(head) + n * size_of(dtype) + kChunkBytes - 1) / kChunkBytes;
 }
 
-// Fills the table from tensor `from` on, skipping empty ones; returns the first tensor that did not fit.
+// Fills the table from tensor `from` on, skipping empty ones; returns the first tensor that did not fit. The list's
+// chunks fit 32 bits (checked by the entry points).
 template <int CAP>
 int fill(Table<CAP>& t, int from, int count, const void* const* src, void* const* dst, const long long* n,
          const unsigned char* dtypes) {
@@ -365,14 +366,12 @@ int fill(Table<CAP>& t, int from, int count, const void* const* src, void* const
     int i = from;
     for (; i < count && t.count < CAP; ++i) {
         if (n[i] == 0) continue;
-        const long long mine = chunks_of(src[i], n[i], dtypes[i]);
-        if (chunks + mine >= (1ll << 32)) break;  // not reached by what a device holds (64 TB)
         t.src[t.count] = src[i];
         t.dst[t.count] = dst ? dst[i] : nullptr;
         t.n[t.count] = n[i];
         t.dtype[t.count] = dtypes[i];
         t.first_chunk[t.count++] = static_cast<uint32_t>(chunks);
-        chunks += mine;
+        chunks += chunks_of(src[i], n[i], dtypes[i]);
     }
     t.chunks = static_cast<uint32_t>(chunks);
     return i;

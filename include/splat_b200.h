@@ -390,7 +390,7 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
  *          1e154 square to infinity
  *   f = min(1, max_norm / (norm + 1e-6)), NaN when the norm is; computed in float64 from the rounded norm
  * A list of `count` tensors is given as host arrays: device pointers (aligned to their type, no other alignment
- * needed), element counts (at most 32 TiB), and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements may have
+ * needed), element counts (less than 32 TiB in all), and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements may have
  * null pointers.
  * The arrays are read during the call only. *norm is device memory: float32, or float64 when norm_is_f64, which a list
  * with a float64 tensor needs.

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import numpy as np
 import pytest
@@ -40,3 +41,16 @@ def test_lean_groups_without_elements(features):
     assert _lean_step([empty, A._LeanGroup(P, P, P, P, 4, 1e-3, 0, 0)]) == ERR_ARG
     assert "bad size" in L.load().splat_last_error().decode()
     assert _lean_step([A._LeanGroup(P, P, P, P, -4, 1e-3, 1, 0)]) == ERR_ARG
+
+
+@pytest.mark.parametrize("entry", ["norm", "clip"])
+@pytest.mark.parametrize("count,gib", [(1000, 70), (999, 70), (481, 70), (2, 20 * 1024), (100_000, 1)])
+def test_lists_beyond_the_chunk_index(entry, count, gib):
+    """A list may name a large tensor many times: past 32 TiB the index of its chunks no longer fits, nor would its
+    launches' partials fit the workspace."""
+    ptrs, sizes, codes = array("Q", [P] * count), array("q", [gib << 28] * count), bytes(count)
+    args = [count, ptrs.buffer_info()[0]] + ([ptrs.buffer_info()[0]] if entry == "clip" else [])
+    args += [sizes.buffer_info()[0], codes, 2] + ([1.0] if entry == "clip" else [])
+    size = L.query("splat_grad_workspace_size", count)
+    assert getattr(L.load(), f"splat_grad_{entry}")(*args, P, 0, P, size, None) == ERR_ARG
+    assert "32 TiB" in L.load().splat_last_error().decode()
