@@ -15,8 +15,8 @@
 // 64% of the issue slots busy: the 32 elements that a thread adds of a chunk carry the search and the chunk's geometry.
 //
 // Clipping reads the gradients again, since the factor needs all of them: 1M Gaussians (236 MB) clipped into other
-// buffers move 3 x 236 MB less the 64 MiB that the norm's pass keeps in the L2 and take 109 us (644 MB in 98 us would be
-// the copy rate); without the kept lines 113.
+// buffers move 3 x 236 MB less the 64 MiB that the norm's pass leaves in the L2 and take 111.3 us (644 MB in 98 us would
+// be the copy rate); where it leaves nothing there in particular 114.5.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -28,8 +28,10 @@ namespace gradnorm {
 
 constexpr int kNormThreads = 512;
 constexpr int kNormBlocks = 4;  // per SM: all its threads
-// What the norm's pass keeps in the L2 for a second one: 64 MiB of its 126 MB (32 MiB: 110.0 us for the 1M Gaussians
-// above, 96 MiB: 108.5, 64 MiB: 107.5).
+// What the norm's pass leaves in the L2 for a second one: 64 MiB of its 126 MB (32 MiB: 113.2 us for the 1M Gaussians
+// above, 96 MiB: 111.6, 64 MiB: 111.3). Those lines have the normal priority and the ones before them leave first. Lines
+// of the highest priority serve the second pass no better (111.7; the dense step of 3M Gaussians 854 us against 858), and
+// stay when the call is over: every later pass over 80 MB took 20 us where it takes 16.5, until gigabytes had gone by.
 constexpr uint32_t kKeepChunks = 4096;
 // Lists of up to 2048 chunks (32 MiB) leave the partials to the blocks that scale or step, each of which reduces them
 // for itself: one launch less, 3 us of the host's time, and on the device 6.5 against 7.4 us for clipping 20 thousand

@@ -187,13 +187,11 @@ __device__ __forceinline__ void add(double& acc, double g) {
 }
 
 // How soon the L2 lets go of the lines that a load brings in.
-enum class Evict { kFirst, kNormal, kLast };
+enum class Evict { kFirst, kNormal };
 
 __device__ __forceinline__ uint64_t l2_policy(Evict e) {
     uint64_t p;
-    if (e == Evict::kLast)
-        asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
-    else if (e == Evict::kNormal)
+    if (e == Evict::kNormal)
         asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
     else
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
@@ -270,8 +268,8 @@ __device__ __forceinline__ void accumulate(const T* src, long long n, uint32_t c
     }
 }
 
-// This thread's share of the sum over chunks team, team + teams, ... of the table. With `keep`, the last so many chunks
-// are kept in the L2 for the pass that follows, and the others leave it first.
+// This thread's share of the sum over chunks team, team + teams, ... of the table. With `keep`, all but the last so many
+// chunks leave the L2 first, so that those are still there for the pass that follows.
 template <int CAP, int NORM>
 __device__ __forceinline__ double accumulate_table(const Table<CAP>& t, uint32_t team, uint32_t teams, int thread,
                                                    uint32_t keep) {
@@ -281,7 +279,7 @@ __device__ __forceinline__ double accumulate_table(const Table<CAP>& t, uint32_t
         const uint32_t chunk = c - t.first_chunk[k];
         const void* src = t.src[k];
         const uint64_t policy =
-            l2_policy(keep == 0 ? Evict::kNormal : t.chunks - c <= keep ? Evict::kLast : Evict::kFirst);
+            l2_policy(keep == 0 || t.chunks - c <= keep ? Evict::kNormal : Evict::kFirst);
         switch (t.dtype[k]) {
             case SPLAT_F32:
                 accumulate<float, NORM>(static_cast<const float*>(src), t.n[k], chunk, thread, policy, acc);
