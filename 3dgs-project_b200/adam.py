@@ -163,6 +163,7 @@ class FusedAdam(torch.optim.Adam):
         by_key: dict[tuple, list] = {}
         grads: list[torch.Tensor] = []  # in the parameters' order, which the clip's sums follow
         masks: dict[tuple, torch.Tensor | None] = {}
+        counters: list[torch.Tensor] = []
         for group in self.param_groups:
             if len(group["params"]) != 1:
                 raise RuntimeError("more than one tensor in group")
@@ -181,9 +182,9 @@ class FusedAdam(torch.optim.Adam):
                 # densification concatenates float32 zeros to the moments, which promotes them; convert back
                 state["exp_avg"] = state["exp_avg"].to(moment_dtype)
                 state["exp_avg_sq"] = state["exp_avg_sq"].to(moment_dtype)
-            state["step"] += 1
+            counters.append(state["step"])
             grad = param.grad if param.grad.is_contiguous() else param.grad.contiguous()
-            step = int(state["step"].item())
+            step = int(state["step"].item()) + 1
             if not self.lean:
                 key = ("dense", step, *group["betas"], group["eps"], param.device)
                 entry = _Group(param.data_ptr(), grad.data_ptr(), state["exp_avg"].data_ptr(),
@@ -204,13 +205,18 @@ class FusedAdam(torch.optim.Adam):
         clip = None
         if self.max_grad_norm is not None:
             clip = self._clip(grads, len(by_key) == 1 and len(grads) <= MAX_GROUPS)
+        for counter in counters:  # once all memory is had: a step that runs out of it has not happened
+            counter += 1
         for key, groups in by_key.items():
             kind, step, b1, b2, eps, dev = key[:6]
             for s in range(0, len(groups), MAX_GROUPS):
                 _launch(kind == "lean", groups[s:s + MAX_GROUPS], step, (b1, b2), eps, masks.get(key), dev, clip)
 
     def _check_clipped(self) -> None:
-        """The clipped step's gradients: one norm is taken over them, on one device."""
+        """The clipped step's limit, which a caller may set anew between steps, and gradients: one norm is taken over
+        them, on one device."""
+        gs_grad.check_max_norm(self.max_grad_norm)
+        gs_grad.norm_code(self.grad_norm_type)
         devices = set()
         for group in self.param_groups:
             for p in group["params"]:
@@ -232,9 +238,9 @@ class FusedAdam(torch.optim.Adam):
         if in_step:
             buffers = gs_grad.scratch(grads[0].get_device(), len(grads))
             self.grad_norm = buffers[0]
-            return norm, self.max_grad_norm, buffers
+            return norm, float(self.max_grad_norm), buffers
         self.grad_norm = gs_grad.grad_norm(grads, self.grad_norm_type)
-        return gs_grad.NORM_GIVEN, self.max_grad_norm, self.grad_norm
+        return gs_grad.NORM_GIVEN, float(self.max_grad_norm), self.grad_norm
 
 
 def _launch(lean: bool, groups: list, step: int, betas, eps: float, visibility, device, clip) -> None:

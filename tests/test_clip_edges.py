@@ -6,9 +6,11 @@ from array import array
 
 import numpy as np
 import pytest
+import torch
 
 from gs_b200 import _lib as L
 from gs_b200 import adam as A
+from gs_b200 import grad as G
 from oracle import adam_oracle as O
 
 OK, ERR_ARG = 0, 1
@@ -54,3 +56,52 @@ def test_lists_beyond_the_chunk_index(entry, count, gib):
     size = L.query("splat_grad_workspace_size", count)
     assert getattr(L.load(), f"splat_grad_{entry}")(*args, P, 0, P, size, None) == ERR_ARG
     assert "32 TiB" in L.load().splat_last_error().decode()
+
+
+@pytest.fixture
+def steps(monkeypatch):
+    """FusedAdam on the CPU up to its launches, which are listed (step, groups, clip) instead of made."""
+    made = []
+    monkeypatch.setattr(A.L, "check_cuda", lambda name, t, dtype=None: t)
+    monkeypatch.setattr(A.FusedAdam, "_check_clipped", lambda self: None)
+    monkeypatch.setattr(A, "_launch", lambda lean, groups, step, betas, eps, visibility, device, clip:
+                        made.append((step, len(groups), clip)))
+    return made
+
+
+@pytest.mark.parametrize("count", [2, 11])
+def test_a_step_that_runs_out_of_memory_is_not_counted(monkeypatch, steps, count):
+    """The buffers of the norm are had before the counters go on (count 11: a norm of its own, for several launches)."""
+    params = [torch.nn.Parameter(torch.ones(3)) for _ in range(count)]
+    for p in params:
+        p.grad = torch.ones(3)
+    opt = A.FusedAdam([{"params": [p]} for p in params], lr=1e-3, eps=1e-15, max_grad_norm=1.0)
+
+    def full(*args):
+        raise torch.OutOfMemoryError("no memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(G, "scratch", full)
+        m.setattr(G, "grad_norm", full)
+        with pytest.raises(torch.OutOfMemoryError):
+            opt.step()
+    assert not steps and all(float(opt.state[p]["step"]) == 0 for p in params)
+    norm = torch.zeros(())
+    monkeypatch.setattr(G, "scratch", lambda *args: (norm, 0, None, 0, 0))
+    monkeypatch.setattr(G, "grad_norm", lambda *args: norm)
+    for n in (1, 2):
+        steps.clear()
+        opt.step()
+        assert all(float(opt.state[p]["step"]) == n for p in params)
+        assert [s[0] for s in steps] == [n] * len(steps) and sum(s[1] for s in steps) == count
+
+
+def test_a_limit_set_between_steps_is_checked():
+    opt = A.FusedAdam([torch.nn.Parameter(torch.zeros(3))], lr=1e-3, eps=1e-15, max_grad_norm=1.0)
+    for bad in (-1.0, float("nan")):
+        opt.max_grad_norm = bad
+        with pytest.raises(ValueError):
+            opt.step()
+    opt.max_grad_norm, opt.grad_norm_type = 2, 3
+    with pytest.raises(ValueError):
+        opt.step()
