@@ -164,6 +164,7 @@ class FusedAdam(torch.optim.Adam):
         grads: list[torch.Tensor] = []  # in the parameters' order, which the clip's sums follow
         masks: dict[tuple, torch.Tensor | None] = {}
         counters: list[torch.Tensor] = []
+        updated: list[torch.Tensor] = []
         for group in self.param_groups:
             if len(group["params"]) != 1:
                 raise RuntimeError("more than one tensor in group")
@@ -183,6 +184,7 @@ class FusedAdam(torch.optim.Adam):
                 state["exp_avg"] = state["exp_avg"].to(moment_dtype)
                 state["exp_avg_sq"] = state["exp_avg_sq"].to(moment_dtype)
             counters.append(state["step"])
+            updated += param, state["exp_avg"], state["exp_avg_sq"]
             grad = param.grad if param.grad.is_contiguous() else param.grad.contiguous()
             step = int(state["step"].item()) + 1
             if not self.lean:
@@ -211,6 +213,8 @@ class FusedAdam(torch.optim.Adam):
             kind, step, b1, b2, eps, dev = key[:6]
             for s in range(0, len(groups), MAX_GROUPS):
                 _launch(kind == "lean", groups[s:s + MAX_GROUPS], step, (b1, b2), eps, masks.get(key), dev, clip)
+        if clip is not None:
+            gs_grad.written(updated)
 
     def _check_clipped(self) -> None:
         """The clipped step's limit, which a caller may set anew between steps, and gradients: one norm is taken over
@@ -293,6 +297,7 @@ def _clipped_step(groups: list[tuple], lean: bool, step: int, betas, eps: float,
     with nullcontext() if current else torch.cuda.device(device):
         L.call("adam_step_multi_lean_clipped" if lean else "adam_step_multi_clipped", *args, code, limit, norm_ptr,
                ws_ptr, ws_bytes, stream)
+    gs_grad.written(groups)
     return norm
 
 

@@ -193,6 +193,27 @@ PyObject* adam_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
 }
 
+void bump(PyObject* item) {
+    if (!THPVariable_Check(item)) return;
+    const at::Tensor& t = THPVariable_Unpack(item);
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // inference tensors count nothing
+}
+
+// written(entries): tells autograd that a kernel wrote the entries, tensors or the groups (param, grad, exp_avg,
+// exp_avg_sq, lr) of a step, so that a backward that saved their old values raises.
+PyObject* written(PyObject*, PyObject* seq) {
+    HANDLE_TH_ERRORS
+    const Entries e(seq);
+    for (Py_ssize_t i = 0; i < e.count; ++i) {
+        const Entries group(e.items[i]);
+        if (group.count == 0) bump(e.items[i]);
+        for (Py_ssize_t k = 0; k < group.count; ++k)
+            if (k != 1) bump(group.items[k]);
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"describe", describe, METH_O, "describe(tensors) -> (addresses, sizes, codes, device, current, stream)"},
     {"same_form", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(same_form)), METH_FASTCALL,
@@ -201,6 +222,7 @@ PyMethodDef kMethods[] = {
      "scratch(device, float64, bytes) -> (norm, address, workspace, address)"},
     {"adam_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adam_table)), METH_FASTCALL,
      "adam_table(groups, lean) -> (table, device, current, stream)"},
+    {"written", written, METH_O, "written(tensors or groups): counts a write for autograd"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

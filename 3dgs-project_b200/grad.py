@@ -9,7 +9,8 @@ The Adam steps of gs_b200.adam take max_grad_norm and clip as they read the grad
 Tensors are float32, bfloat16, float16 or float64 CUDA tensors, mixed in one call, each dense in its own order of
 dimensions (contiguous, transposed, channels-last), of any length and at any address. Sums are taken in float64 in an
 order that the sizes fix, so a call repeats bit for bit. None of the calls waits for the device (error_if_nonfinite
-apart), and all can be captured into a CUDA graph. Nothing is recorded for autograd.
+apart), and all can be captured into a CUDA graph. Nothing is recorded for autograd, except that tensors were written: as
+after torch's own in-place operations, a backward that needs their old values raises.
 """
 from __future__ import annotations
 
@@ -144,6 +145,11 @@ def adam_table(groups: list, lean: bool):
     return _tensors().adam_table(groups, lean)
 
 
+def written(entries) -> None:
+    """Counts a write of the tensors (of a step's groups: of parameters and moments) for autograd."""
+    _tensors().written(entries)
+
+
 def _norm(d: Described, norm: int) -> torch.Tensor:
     f64 = 3 in d.codes
     count = len(d.codes)
@@ -208,6 +214,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         norm, norm_ptr, ws_ptr, ws_bytes = NORM_GIVEN, read.data_ptr(), None, 0
     d.call("splat_grad_clip", count, d.addresses, to.addresses, d.sizes, d.codes, norm, limit, norm_ptr, f64, ws_ptr,
            ws_bytes)
+    if out is not None:
+        written(outs)
     return list(outs), total_norm
 
 

@@ -105,3 +105,14 @@ def test_a_limit_set_between_steps_is_checked():
     opt.max_grad_norm, opt.grad_norm_type = 2, 3
     with pytest.raises(ValueError):
         opt.step()
+
+
+def test_writes_are_counted_for_autograd():
+    x, y, g = torch.zeros(3), torch.zeros(2, 2)[0], torch.ones(3)
+    with torch.inference_mode():
+        quiet = torch.zeros(3)
+    G.written([x, y, quiet, "x"])
+    assert x._version == 1 and y._version == 1
+    G.written([(x, g, y, [1], 1e-3), [y, g]])
+    assert x._version == 2 and y._version == 3 and g._version == 0
+    G.written([])

@@ -127,3 +127,43 @@ def test_the_cache_is_left_to_others(cuda, call):
 
     calls[call]()
     assert passes(calls[call]) <= 1.1 * passes(lambda: None)
+
+
+def test_a_backward_through_what_was_clipped_raises(cuda):
+    """As after torch's clipping: a second derivative that needs the raw gradient must not take the clipped one."""
+    x = torch.randn(2000, device=cuda, requires_grad=True)
+    for call in (lambda: G.clip_grad_norm_([x], 0.1), lambda: G.clip_grads([x.grad.detach()], 0.1, out=[x.grad.detach()]),
+                 lambda: G.clip_grad_norm_([x], 0.1, error_if_nonfinite=True)):
+        x.grad, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+        again = (x.grad ** 2).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            again.backward()
+    x.grad, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    again = (x.grad ** 2).sum()
+    G.clip_grads([x.grad], 0.1)  # into new tensors: nothing is lost
+    G.grad_norm([x.grad])
+    second, = torch.autograd.grad(again, x)
+    assert torch.equal(second, torch.autograd.grad(((3 * x * x) ** 2).sum(), x)[0])
+    with torch.inference_mode():
+        quiet = torch.randn(2000, device=cuda)
+    G.clip_grads([quiet], 0.1, out=[quiet])
+
+
+@pytest.mark.parametrize("lean", [False, True])
+def test_a_backward_through_what_was_stepped_raises(cuda, lean):
+    step = A.adam_step_lean if lean else A.adam_step
+    groups = adam_state(50, cuda, 1)
+    p = groups[0][0].requires_grad_()
+    loss = (p ** 2).sum()
+    step(groups, 1, max_grad_norm=1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    p = torch.randn(50, 3, device=cuda, requires_grad=True)
+    opt = A.FusedAdam([{"params": [p], "name": "p"}], lr=1e-3, eps=1e-15, max_grad_norm=1.0,
+                      lowp_moment_groups=("p",) if lean else ())
+    loss = (p ** 2).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
