@@ -307,7 +307,7 @@ def adam_step(groups: list[tuple], step: int, betas=(0.9, 0.999), eps: float = 1
 
     With max_grad_norm the step takes the gradients times min(1, max_grad_norm / (norm + 1e-6)), norm the global norm
     of order norm_type (1, 2 or inf) over the groups' gradients, and returns the norm (0-d, on the device). The
-    gradients keep their values."""
+    gradients keep their values, and may share no memory with what is written; nor may the groups, among themselves."""
     if not groups:
         return None if max_grad_norm is None else torch.zeros(())
     if max_grad_norm is not None:

@@ -512,6 +512,29 @@ struct Grads {
     unsigned char dtype[SPLAT_ADAM_MAX_GROUPS];
 };
 
+unsigned long long moment_bytes(const adam_group&) { return 4; }
+unsigned long long moment_bytes(const adam_lean_group& g) { return g.lowp_moments ? 2 : 4; }
+
+// What a clipped step writes overlaps nothing else of it: in a step of one launch some clusters still read the gradients
+// for the norm while others write.
+template <typename G>
+int check_overlap(const char* what, int count, const G* groups, const float* norm, bool given) {
+    gradnorm::Range s[4 * SPLAT_ADAM_MAX_GROUPS + 1];
+    int k = 0;
+    s[k++] = gradnorm::range_of(norm, sizeof(float), !given);
+    for (int i = 0; i < count; ++i) {
+        const G& g = groups[i];
+        if (g.n == 0) continue;
+        const auto n = static_cast<unsigned long long>(g.n);
+        s[k++] = gradnorm::range_of(g.param, 4 * n, true);
+        s[k++] = gradnorm::range_of(g.grad, 4 * n, false);
+        s[k++] = gradnorm::range_of(g.exp_avg, moment_bytes(g) * n, true);
+        s[k++] = gradnorm::range_of(g.exp_avg_sq, moment_bytes(g) * n, true);
+    }
+    SPLAT_REQUIRE(gradnorm::apart(s, k), "%s: a buffer that is written overlaps another one of the call", what);
+    return SPLAT_OK;
+}
+
 // A clipped step: the norm's kernel and the update's, or for a small model one kernel that does both.
 template <typename G, typename T>
 int clipped_step(const char* what, int count, const G* groups, const T& table, long long blocks,
@@ -525,6 +548,7 @@ int clipped_step(const char* what, int count, const G* groups, const T& table, l
     SPLAT_REQUIRE(
         given || (gradnorm::aligned(workspace, true) && workspace_bytes >= splat_grad_workspace_size(count)),
         "%s: workspace too small or not aligned", what);
+    SPLAT_TRY(check_overlap(what, count, groups, norm, given));
     if (blocks == 0)  // the norm of nothing is the call's all the same
         return given ? SPLAT_OK
                      : splat_grad_norm(0, nullptr, nullptr, nullptr, norm_type, norm, 0, workspace, workspace_bytes,

@@ -286,34 +286,20 @@ int check_list(const char* what, int count, const void* const* grads, const long
     return SPLAT_OK;
 }
 
-struct Range {
-    uintptr_t begin, end;
-    bool written;
-};
-
 // What is written overlaps nothing else: the outputs one another, (out of place) any input, or the norm.
 int check_overlap(int count, const void* const* grads, void* const* outs, const long long* n,
                   const unsigned char* dtypes, bool in_place, const Clip& c, bool given) {
     std::unique_ptr<Range[]> s(new (std::nothrow) Range[2 * static_cast<size_t>(count) + 1]);
     SPLAT_REQUIRE(s, "splat_grad_clip: out of host memory");
     int k = 0;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(c.norm);
-    s[k++] = {at, at + (c.norm_f64 ? 8u : 4u), !given};
+    s[k++] = range_of(c.norm, c.norm_f64 ? 8 : 4, !given);
     for (int i = 0; i < count; ++i) {
         if (n[i] == 0) continue;
-        const uintptr_t bytes = static_cast<uintptr_t>(n[i]) * size_of(dtypes[i]);
-        const uintptr_t o = reinterpret_cast<uintptr_t>(outs[i]), g = reinterpret_cast<uintptr_t>(grads[i]);
-        s[k++] = {o, o + bytes, true};
-        if (!in_place) s[k++] = {g, g + bytes, false};
+        const auto bytes = static_cast<unsigned long long>(n[i]) * size_of(dtypes[i]);
+        s[k++] = range_of(outs[i], bytes, true);
+        if (!in_place) s[k++] = range_of(grads[i], bytes, false);
     }
-    std::sort(s.get(), s.get() + k, [](const Range& a, const Range& b) { return a.begin < b.begin; });
-    uintptr_t written_to = 0, read_to = 0;
-    for (int i = 0; i < k; ++i) {
-        SPLAT_REQUIRE(s[i].begin >= written_to && (!s[i].written || s[i].begin >= read_to),
-                      "splat_grad_clip: a tensor that is written overlaps another one of the call");
-        uintptr_t& to = s[i].written ? written_to : read_to;
-        to = std::max(to, s[i].end);
-    }
+    SPLAT_REQUIRE(apart(s.get(), k), "splat_grad_clip: a tensor that is written overlaps another one of the call");
     return SPLAT_OK;
 }
 

@@ -10,6 +10,8 @@
 //   factor = min(1, max_norm / (norm + 1e-6)) in float64 from the rounded norm; NaN where the norm is NaN
 #pragma once
 
+#include <algorithm>
+
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -348,6 +350,29 @@ inline int size_of(int dtype) { return dtype == SPLAT_F32 ? 4 : dtype == SPLAT_F
 
 // A buffer of float32 or float64 values that is there.
 inline bool aligned(const void* p, bool f64) { return p && reinterpret_cast<uintptr_t>(p) % (f64 ? 8 : 4) == 0; }
+
+// A buffer of a call.
+struct Range {
+    uintptr_t begin, end;
+    bool written;
+};
+
+inline Range range_of(const void* p, unsigned long long bytes, bool written) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return {at, at + bytes, written};
+}
+
+// No range that is written overlaps another one. Sorts them.
+inline bool apart(Range* s, int count) {
+    std::sort(s, s + count, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t written_to = 0, read_to = 0;
+    for (int i = 0; i < count; ++i) {
+        if (s[i].begin < written_to || (s[i].written && s[i].begin < read_to)) return false;
+        uintptr_t& to = s[i].written ? written_to : read_to;
+        to = std::max(to, s[i].end);
+    }
+    return true;
+}
 
 inline long long chunks_of(const void* src, long long n, int dtype) {
     const uintptr_t head = reinterpret_cast<uintptr_t>(src) & (kVecBytes - 1);

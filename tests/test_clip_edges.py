@@ -116,3 +116,33 @@ def test_writes_are_counted_for_autograd():
     G.written([(x, g, y, [1], 1e-3), [y, g]])
     assert x._version == 2 and y._version == 3 and g._version == 0
     G.written([])
+
+
+def _clipped(lean, groups, norm=64 * P, norm_type=2):
+    cls = A._LeanGroup if lean else A._Group
+    arr = (cls * len(groups))(*[cls(*g, 1e-3, 1, int(lean)) if lean else cls(*g, 1e-3) for g in groups])
+    head = (len(groups), ctypes.addressof(arr), 1, 0.9, 0.999, 1e-15)
+    tail = (norm_type, 1.0, norm, 128 * P, 1 << 20, None)
+    lib = L.load()
+    return lib.adam_step_multi_lean_clipped(*head, None, 0, *tail) if lean else lib.adam_step_multi_clipped(*head, *tail)
+
+
+FIRST, SECOND = (P, 2 * P, 3 * P, 4 * P, 64), (5 * P, 6 * P, 7 * P, 8 * P, 64)
+
+
+@pytest.mark.parametrize("lean", [False, True])
+@pytest.mark.parametrize("groups,kw", [
+    ([(P, P, 3 * P, 4 * P, 64)], {}),                              # the gradient is the parameter
+    ([(P, 3 * P + 64, 3 * P, 4 * P, 64)], {}),                     # lies in the first moment
+    ([(P, 2 * P, 3 * P, 3 * P, 64)], {}),                          # one buffer for both moments
+    ([FIRST, (P, *SECOND[1:])], {}),                               # one parameter in two groups
+    ([FIRST, (P + 128, *SECOND[1:])], {}),                         # two that share elements
+    ([FIRST, (5 * P, P + 240, *SECOND[2:])], {}),                  # a gradient inside the other group's parameter
+    ([FIRST, (*SECOND[:2], 4 * P + 96, *SECOND[3:])], {}),
+    ([FIRST, SECOND], {"norm": 2 * P + 16}),                       # the norm, written over a gradient
+    ([FIRST, SECOND], {"norm": 5 * P, "norm_type": 3}),            # read from a parameter
+])
+def test_a_clipped_step_on_buffers_that_overlap(lean, groups, kw):
+    # a moment's 64 elements have 128 bytes in the lean step here, 256 in the dense one
+    assert _clipped(lean, groups, **kw) == ERR_ARG
+    assert "overlaps" in L.load().splat_last_error().decode()

@@ -168,3 +168,20 @@ def test_a_backward_through_what_was_stepped_raises(cuda, lean):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("n", [512, 300_000])
+def test_groups_side_by_side_in_memory(cuda, n):
+    """Buffers that touch do not overlap, and two groups may take one gradient."""
+    flat = torch.rand(7 * n, device=cuda) + 0.1
+    p0, p1, m0, m1, v0, v1, g = flat.view(7, n)
+    groups = [(p0, g, m0, v0, 1e-3), (p1, g, m1, v1, 1e-2)]
+    other = copies(groups)
+    total = A.adam_step(groups, 3, max_grad_norm=0.5)
+    (a, b), want = G.clip_grads([x[1] for x in other], 0.5)
+    A.adam_step([(x[0], c, *x[2:]) for x, c in zip(other, (a, b))], 3)
+    assert torch.equal(total, want)
+    for x, y in zip(groups, other):
+        assert all(torch.equal(x[i], y[i]) for i in range(4))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        A.adam_step([(p0, p0, m0, v0, 1e-3)], 3, max_grad_norm=0.5)
