@@ -287,6 +287,10 @@ def _clipped_step(groups: list[tuple], lean: bool, step: int, betas, eps: float,
     """adam_step / adam_step_lean with max_grad_norm: the buffers of all groups read and checked in one go."""
     code, limit = gs_grad.norm_code(norm_type), gs_grad.check_max_norm(max_grad_norm)
     read = gs_grad.adam_table(groups, lean)
+    if read is None:  # a rate may be another kind of number
+        held = [tuple(group) for group in groups]
+        groups = [(p, g, m, v, float(lr)) for p, g, m, v, lr in held]
+        read = gs_grad.adam_table(groups, lean)
     if read is None:
         _refuse_groups(groups, lean)
     table, device, current, stream = read

@@ -129,7 +129,7 @@ PyObject* scratch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // adam_table(groups, lean) -> (adam_group or adam_lean_group array as bytes, device index, whether that is the current
 // device, its current stream) for groups (param, grad, exp_avg, exp_avg_sq, lr) of contiguous CUDA tensors of one size
-// on one device: float32, or for the lean table both moments bfloat16. None where a group is not that.
+// on one device: float32, or for the lean table both moments bfloat16; lr a Python float. None where a group is not that.
 // A parameter that appears twice raises.
 PyObject* adam_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (nargs != 2) {
@@ -168,8 +168,8 @@ PyObject* adam_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (kind[0] != at::kFloat || kind[1] != at::kFloat || kind[2] != kind[3] ||
                 !(kind[2] == at::kFloat || (lean && low)))
                 Py_RETURN_NONE;
-            const double lr = PyFloat_AsDouble(g.items[4]);
-            if (lr == -1.0 && PyErr_Occurred()) return nullptr;
+            if (!PyFloat_Check(g.items[4])) Py_RETURN_NONE;  // anything else may run code that changes the lists
+            const double lr = PyFloat_AS_DOUBLE(g.items[4]);
             params[i] = n > 0 ? at[0] : nullptr;
             for (Py_ssize_t j = 0; j < i; ++j)
                 if (params[i] && params[i] == params[j]) {

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -185,3 +186,23 @@ def test_groups_side_by_side_in_memory(cuda, n):
         assert all(torch.equal(x[i], y[i]) for i in range(4))
     with pytest.raises(RuntimeError, match="overlaps"):
         A.adam_step([(p0, p0, m0, v0, 1e-3)], 3, max_grad_norm=0.5)
+
+
+def test_rates_of_other_kinds(cuda):
+    """A rate is anything that float() takes; what its conversion does to the caller's list changes nothing."""
+
+    class Rate:
+        def __float__(self):
+            groups.clear()
+            return 2e-3
+
+    want = adam_state(100, cuda, 2)[:3]
+    A.adam_step([(*x[:4], lr) for x, lr in zip(want, (1.0, 2e-3, 0.5))], 2, max_grad_norm=0.1)
+    for rates in ((1, Rate(), 0.5), (torch.ones((), device=cuda), np.float64(2e-3), np.float32(0.5))):
+        kept = adam_state(100, cuda, 2)[:3]
+        groups = [[*x[:4], lr] for x, lr in zip(kept, rates)]
+        A.adam_step(groups, 2, max_grad_norm=0.1)
+        for x, y in zip(kept, want):
+            assert all(torch.equal(x[i], y[i]) for i in range(4))
+    with pytest.raises((TypeError, ValueError)):
+        A.adam_step([(*want[0][:4], "fast")], 2, max_grad_norm=0.1)
