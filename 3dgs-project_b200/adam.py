@@ -277,6 +277,8 @@ def _refuse_groups(groups: list[tuple], lean: bool) -> None:
             if t.dtype not in moments or (t is v and t.dtype != m.dtype):
                 raise RuntimeError(f"moments of group {i} must be float32" + (", or both bfloat16" if lean else
                                    " (adam_step_lean takes bfloat16 ones)"))
+            if t.is_neg():
+                raise RuntimeError(f"{name} of group {i} is a view that negates its memory: call resolve_neg()")
             if t.numel() != p.numel() or t.device != groups[0][0].device:
                 raise RuntimeError(f"{name} of group {i} must have its parameter's size, on the first group's device")
     raise RuntimeError("the groups cannot be read as dense CUDA tensors")

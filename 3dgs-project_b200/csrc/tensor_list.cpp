@@ -45,7 +45,8 @@ struct Entries {
 
 // describe(list or tuple) -> (addresses uint64, element counts int64, type codes uint8, device index, whether that is
 // the current device, its current stream), the first three as bytes, when every entry is a dense
-// strided CUDA tensor of a known type, all on one device; otherwise None (the caller then says which is not, and why).
+// strided CUDA tensor of a known type whose memory holds its values (no lazy negation), all on one device; otherwise
+// None (the caller then says which is not, and why).
 PyObject* describe(PyObject*, PyObject* seq) {
     const Entries e(seq);
     if (e.count == 0) Py_RETURN_NONE;
@@ -57,7 +58,7 @@ PyObject* describe(PyObject*, PyObject* seq) {
         for (Py_ssize_t i = 0; i < e.count; ++i) {
             if (!THPVariable_Check(e.items[i])) Py_RETURN_NONE;
             const at::Tensor& t = THPVariable_Unpack(e.items[i]);
-            if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided) Py_RETURN_NONE;
+            if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_neg()) Py_RETURN_NONE;
             const int c = code_of(t.scalar_type());
             if (c < 0 || (i > 0 && t.get_device() != device)) Py_RETURN_NONE;
             device = static_cast<int>(t.get_device());
@@ -153,7 +154,8 @@ PyObject* adam_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             for (int k = 0; k < 4; ++k) {
                 if (!THPVariable_Check(g.items[k])) Py_RETURN_NONE;
                 const at::Tensor& t = THPVariable_Unpack(g.items[k]);
-                if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous()) Py_RETURN_NONE;
+                if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.is_contiguous() || t.is_neg())
+                    Py_RETURN_NONE;
                 if (i == 0 && k == 0) device = t.get_device();
                 if (k == 0) {
                     n = t.numel();

@@ -62,6 +62,8 @@ def _refuse(name: str, tensors: list) -> None:
         if t.layout != torch.strided or t.dtype not in _CODES:
             raise RuntimeError(f"{name}[{i}] must be a dense float32, bfloat16, float16 or float64 tensor, got "
                                f"{t.dtype} ({t.layout})")
+        if t.is_neg():
+            raise RuntimeError(f"{name}[{i}] is a view that negates its memory (of a conjugate): call resolve_neg()")
         if t.numel() and not t.is_contiguous() and not _dense(t):
             raise RuntimeError(f"{name}[{i}] must be dense (contiguous, or contiguous with its dimensions in another "
                                f"order), got shape {tuple(t.shape)} with strides {t.stride()}")
@@ -209,7 +211,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
         if total_norm.dtype not in (torch.float32, torch.float64) or total_norm.numel() != 1 \
                 or total_norm.get_device() != d.device:
             raise RuntimeError("total_norm must be one float32 or float64 value on the gradients' device")
-        read = total_norm.detach().double() if f64 else total_norm
+        read = total_norm.detach().resolve_neg()
+        read = read.double() if f64 else read
         f64 = read.dtype == torch.float64
         norm, norm_ptr, ws_ptr, ws_bytes = NORM_GIVEN, read.data_ptr(), None, 0
     d.call("splat_grad_clip", count, d.addresses, to.addresses, d.sizes, d.codes, norm, limit, norm_ptr, f64, ws_ptr,

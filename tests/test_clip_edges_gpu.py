@@ -206,3 +206,17 @@ def test_rates_of_other_kinds(cuda):
             assert all(torch.equal(x[i], y[i]) for i in range(4))
     with pytest.raises((TypeError, ValueError)):
         A.adam_step([(*want[0][:4], "fast")], 2, max_grad_norm=0.1)
+
+
+def test_views_that_negate_their_memory(cuda):
+    """The imaginary part of a lazy conjugate: its memory holds the values of the other sign."""
+    z = torch.complex(torch.ones(1, device=cuda), torch.full((1,), 2.0, device=cuda))
+    g, plain = z.conj().imag, torch.ones(1, device=cuda)
+    assert g.is_neg() and g.is_contiguous() and float(g) == -2.0
+    for call in (lambda: G.grad_norm([g]), lambda: G.clip_grads([g], 1.0), lambda: G.clip_grads([plain], 1.0, out=[g]),
+                 lambda: A.adam_step([(plain, g, plain.clone(), plain.clone(), 1e-3)], 1, max_grad_norm=1.0)):
+        with pytest.raises(RuntimeError, match="negates"):
+            call()
+    assert float(G.clip_grads([g.resolve_neg()], 1.0)[0][0]) == pytest.approx(-1.0, rel=1e-5)
+    total = torch.complex(plain, -4.0 * plain).conj().imag  # 4
+    assert float(G.clip_grads([plain], 1.0, total_norm=total)[0][0]) == pytest.approx(0.25, rel=1e-5)
