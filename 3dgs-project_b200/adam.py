@@ -228,6 +228,8 @@ class FusedAdam(torch.optim.Adam):
                     L.check_cuda("param", p, torch.float32)
                     if p.grad.dtype != torch.float32 or not p.grad.is_cuda or p.grad.layout != torch.strided:
                         raise RuntimeError("max_grad_norm needs dense float32 CUDA gradients")
+                    if p.grad.is_neg():
+                        raise RuntimeError("a gradient is a view that negates its memory: call resolve_neg()")
                     devices.add(p.device)
         if len(devices) > 1:
             raise RuntimeError("max_grad_norm needs the parameters on one device")

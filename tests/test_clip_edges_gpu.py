@@ -218,5 +218,10 @@ def test_views_that_negate_their_memory(cuda):
         with pytest.raises(RuntimeError, match="negates"):
             call()
     assert float(G.clip_grads([g.resolve_neg()], 1.0)[0][0]) == pytest.approx(-1.0, rel=1e-5)
+    p = torch.ones(1, device=cuda, requires_grad=True)
+    p.grad = g
+    opt = A.FusedAdam([{"params": [p]}], lr=1e-3, eps=1e-15, max_grad_norm=1.0)
+    with pytest.raises(RuntimeError, match="negates"):
+        opt.step()
     total = torch.complex(plain, -4.0 * plain).conj().imag  # 4
     assert float(G.clip_grads([plain], 1.0, total_norm=total)[0][0]) == pytest.approx(0.25, rel=1e-5)
