@@ -222,10 +222,11 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_n
     return list(outs), total_norm
 
 
-def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                    foreach: bool | None = None) -> torch.Tensor:
     """Scales the parameters' gradients in place so that their norm together is at most max_norm, and returns the norm
-    they had (torch.nn.utils.clip_grad_norm_'s call). Parameters without a gradient are passed over; one gradient may
+    they had (torch.nn.utils.clip_grad_norm_'s call, for dense gradients on one CUDA device; foreach chooses between
+    torch's implementations and changes nothing here). Parameters without a gradient are passed over; one gradient may
     not appear twice. error_if_nonfinite raises for an infinite or NaN norm, before anything is scaled (which waits
     for the device)."""
     norm_code(norm_type), check_max_norm(max_norm)

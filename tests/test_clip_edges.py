@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import inspect
 from array import array
 
 import numpy as np
@@ -146,3 +147,12 @@ def test_a_clipped_step_on_buffers_that_overlap(lean, groups, kw):
     # a moment's 64 elements have 128 bytes in the lean step here, 256 in the dense one
     assert _clipped(lean, groups, **kw) == ERR_ARG
     assert "overlaps" in L.load().splat_last_error().decode()
+
+
+def test_the_call_of_torch():
+    """clip_grad_norm_ takes what torch's takes, in torch's order."""
+    ours, torchs = (list(inspect.signature(f).parameters.values())
+                    for f in (G.clip_grad_norm_, torch.nn.utils.clip_grad_norm_))
+    assert [(p.name, p.default) for p in ours] == [(p.name, p.default) for p in torchs]
+    for foreach in (None, True, False):
+        assert float(G.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0, foreach=foreach)) == 0.0
