@@ -1,4 +1,5 @@
 """Builds libsplat_b200.so (all csrc/*.cu for sm_100a, nvcc) and _tensors.so (csrc/tensor_list.cpp, g++) in place.
+The first needs the CUDA toolkit only; the second is passed over where torch or Python's headers are absent.
 
     python 3dgs-project_b200/build.py [--force] [--verbose]
 
@@ -47,12 +48,22 @@ def _digest(sources: list[Path]) -> str:
     return h.hexdigest()
 
 
-def build_tensors(force: bool = False, verbose: bool = False) -> Path:
-    """The host-only module that reads lists of torch tensors: g++ against this interpreter's and torch's headers."""
-    torch_dir = Path(importlib.util.find_spec("torch").submodule_search_locations[0])
+def python_header() -> Path:
+    return Path(sysconfig.get_paths()["include"]) / "Python.h"
+
+
+def build_tensors(force: bool = False, verbose: bool = False) -> Path | None:
+    """The host-only module that reads lists of torch tensors: g++ against this interpreter's and torch's headers. None
+    where these are absent: the Python package cannot be used there (its calls on lists say so), the C ABI can."""
+    torch = importlib.util.find_spec("torch")
+    absent = "torch" if torch is None else "Python.h" if not python_header().exists() else None
+    if absent:
+        print(f"{TENSORS.name} is not built: {absent} is absent", file=sys.stderr)
+        return None
+    torch_dir = Path(torch.submodule_search_locations[0])
     src = CSRC / "tensor_list.cpp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", str(src), f"-I{torch_dir / 'include'}",
-           f"-I{torch_dir / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{torch_dir / 'include/torch/csrc/api/include'}", f"-I{python_header().parent}",
            f"-I{Path(nvcc()).resolve().parent.parent / 'include'}", f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch_python"]
     version = (torch_dir / "version.py").read_bytes()
@@ -74,7 +85,13 @@ def build_tensors(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
+    lib = build_library(force, verbose)
     build_tensors(force, verbose)
+    return lib
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """The C ABI library."""
     sources = sorted(CSRC.glob("*.cu"))
     stamp = BUILD / "stamp"
     digest = _digest(sources)

@@ -2,8 +2,10 @@
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import inspect
 from array import array
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -156,3 +158,40 @@ def test_the_call_of_torch():
     assert [(p.name, p.default) for p in ours] == [(p.name, p.default) for p in torchs]
     for foreach in (None, True, False):
         assert float(G.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0, foreach=foreach)) == 0.0
+
+
+@pytest.fixture
+def builder():
+    path = Path(L.__file__).with_name("build.py")
+    spec = importlib.util.spec_from_file_location("builder_under_test", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+@pytest.mark.parametrize("absent", ["torch", "Python.h"])
+def test_the_library_builds_without_torch(monkeypatch, tmp_path, capsys, builder, absent):
+    """Without torch, or Python's headers, the C ABI library is built and the module that reads tensors is not."""
+    monkeypatch.setattr(builder, "TENSORS", tmp_path / "_tensors.so")
+    if absent == "torch":
+        find = importlib.util.find_spec
+        monkeypatch.setattr(importlib.util, "find_spec", lambda name: None if name == "torch" else find(name))
+    else:
+        monkeypatch.setattr(builder.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    assert builder.build() == builder.LIB and builder.LIB.exists()
+    assert not builder.TENSORS.exists() and f"{absent} is absent" in capsys.readouterr().err
+
+
+def test_the_library_is_built_first(monkeypatch, builder):
+    """A module that does not compile stops the build with an error that names it, after the library."""
+    order = []
+    monkeypatch.setattr(builder, "build_library", lambda *a: order.append("library"))
+
+    def fails(*args):
+        order.append("tensors")
+        raise RuntimeError("g++ failed on tensor_list.cpp")
+
+    monkeypatch.setattr(builder, "build_tensors", fails)
+    with pytest.raises(RuntimeError, match="tensor_list.cpp"):
+        builder.build()
+    assert order == ["library", "tensors"]
