@@ -7,7 +7,8 @@
 // block that uses the norm, reduces the few hundred of them in an order that depends on their number only. A short list
 // takes one launch, in which the blocks of a cluster exchange their partials.
 //   norm = sqrt(sum), sum or max, rounded once to the caller's type (float32, or float64)
-//   factor = min(1, max_norm / (norm + 1e-6)) in float64 from the rounded norm; NaN where the norm is NaN
+//   factor = min(1, max_norm / (norm + 1e-6)) in float64 from the rounded norm; NaN where the norm is NaN, or infinite
+//            like max_norm
 #pragma once
 
 #include <algorithm>

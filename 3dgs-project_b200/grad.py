@@ -8,9 +8,11 @@ The Adam steps of gs_b200.adam take max_grad_norm and clip as they read the grad
 
 Tensors are float32, bfloat16, float16 or float64 CUDA tensors, mixed in one call, each dense in its own order of
 dimensions (contiguous, transposed, channels-last), of any length and at any address. Sums are taken in float64 in an
-order that the sizes fix, so a call repeats bit for bit. None of the calls waits for the device (error_if_nonfinite
-apart), and all can be captured into a CUDA graph. Nothing is recorded for autograd, except that tensors were written: as
-after torch's own in-place operations, a backward that needs their old values raises.
+order that follows from the list's lengths and types, the addresses modulo 16 bytes and the device, so a call on the same
+tensors repeats bit for bit; copies at other addresses may differ in the last bits of the float64 sum. None of the calls
+waits for the device (error_if_nonfinite apart), and all can be captured into a CUDA graph. Nothing is recorded for
+autograd, except that tensors were written: as after torch's own in-place operations, a backward that needs their old
+values raises.
 """
 from __future__ import annotations
 
@@ -168,7 +170,8 @@ def _check_finite(norm: torch.Tensor, norm_type) -> None:
 
 def grad_norm(grads, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """The norm of all elements of the tensors as one vector: 0-d, float32 (float64 when one of them is float64), on
-    their device. norm_type: 1, 2 or inf. NaN when an element is NaN. No tensors: 0 on the CPU, as torch's clipping
+    their device. norm_type: 1, 2 or inf. NaN when an element is NaN. Squares of float64 elements leave float64's range
+    beyond 1e154 (the norm is infinite) and below 1e-162 (they count as 0); those of the other types do not. No tensors: 0 on the CPU, as torch's clipping
     gives. error_if_nonfinite raises for an infinite or NaN norm (which waits for the device)."""
     norm = norm_code(norm_type)
     tensors = _listed(grads)
@@ -181,8 +184,10 @@ def grad_norm(grads, norm_type: float = 2.0, error_if_nonfinite: bool = False) -
 
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None, total_norm: torch.Tensor | None = None):
-    """(clipped, total_norm): the gradients times min(1, max_norm / (total_norm + 1e-6)), each rounded once to its own
-    type. A NaN norm makes them all NaN; an infinite one makes them 0, and NaN where they are infinite.
+    """(clipped, total_norm): the gradients times min(1, max_norm / (total_norm + 1e-6)). The factor is taken in float64
+    and rounded to float32 for all but float64 gradients; the product of a 16-bit gradient is taken in float32 and rounded
+    to its type. A NaN norm makes them all NaN; an infinite one makes them 0, and NaN where they are infinite, unless
+    max_norm is infinite too: then they are all NaN (as torch's clipping gives).
 
     out: the tensors to write, of the gradients' shapes, types and strides; they may not overlap the gradients or one
     another. None makes new ones; `out=grads` (or the same tensors) clips in place, where a norm below max_norm writes

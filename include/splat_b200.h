@@ -43,8 +43,9 @@ long long splat_launch_count(void);
  * library records begin_event just before and end_event just after every launch of `kernel`, on the stream it
  * launches on (cudaEvent_t handles created by the caller, passed as void*; NULL events stop the timing). Kernels:
  * "k_preprocess", "k_duplicate", "k_blend" (training and render-only forward), "k_blend_backward",
- * "k_preprocess_backward", "k_adam" (the clipped steps' update too), "gs2d_k_render" (gs2d forward), "gs2d_k_backward_splat". At most four
- * kernels at once. The events are re-recorded by every launch: read them before the kernel runs again. */
+ * "k_preprocess_backward", "k_adam" (the clipped steps' update too), "gs2d_k_render" (gs2d forward),
+ * "gs2d_k_backward_splat". At most four kernels at once. The events are re-recorded by every launch: read them before
+ * the kernel runs again. */
 int splat_time_kernel(const char* kernel, void* begin_event, void* end_event);
 
 /* ---------------------------------------------------------------------------------------------
@@ -386,16 +387,18 @@ int adam_step_multi_lean(int count, const adam_lean_group* groups, int step, dou
 /* ---------------------------------------------------------------------------------------------
  * Global gradient norm, clipping by it, and the Adam steps that clip (no counterpart in the reference).
  *   norm = (sum |g|^p)^(1/p) over every element of every tensor, p = 1 or 2, or max |g|; sums in float64, in an order
- *          fixed by the sizes (the same call gives the same bits); NaN when an element is NaN; float64 elements beyond
- *          1e154 square to infinity
- *   f = min(1, max_norm / (norm + 1e-6)), NaN when the norm is; computed in float64 from the rounded norm
+ *          that follows from the sizes, types, addresses modulo 16 bytes and the device (the same call gives the same
+ *          bits); NaN when an element is NaN; squares of float64 elements beyond 1e154 are infinite, below 1e-162 they
+ *          are 0
+ *   f = min(1, max_norm / (norm + 1e-6)) in float64 from the rounded norm; NaN when the norm is NaN, or infinite like
+ *       max_norm
  * A list of `count` tensors is given as host arrays: device pointers (aligned to their type, no other alignment
- * needed), element counts (less than 32 TiB in all), and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements may have
- * null pointers.
- * The arrays are read during the call only. *norm is device memory: float32, or float64 when norm_is_f64, which a list
- * with a float64 tensor needs.
- * workspace: device scratch of splat_grad_workspace_size(count) bytes, 8-byte aligned, not kept between calls; calls that may run at
- * the same time (other streams, graphs replayed side by side) need one each.
+ * needed), element counts (less than 32 TiB in all), and SPLAT_F32 ... SPLAT_F64 per tensor; tensors without elements
+ * may have null pointers. The arrays are read during the call only. *norm is device memory: float32, or float64 when
+ * norm_is_f64, which a list with a float64 tensor needs.
+ * workspace: device scratch of splat_grad_workspace_size(count) bytes, 8-byte aligned, apart from the call's other
+ * buffers, not kept between calls; calls that may run at the same time (other streams, graphs replayed side by side)
+ * need one each.
  * ------------------------------------------------------------------------------------------- */
 #define SPLAT_F32 0
 #define SPLAT_BF16 1

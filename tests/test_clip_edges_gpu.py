@@ -225,3 +225,31 @@ def test_views_that_negate_their_memory(cuda):
         opt.step()
     total = torch.complex(plain, -4.0 * plain).conj().imag  # 4
     assert float(G.clip_grads([plain], 1.0, total_norm=total)[0][0]) == pytest.approx(0.25, rel=1e-5)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0])
+@pytest.mark.parametrize("n", [900, 60_000, 3_000_017])
+def test_every_bit_of_a_float64_norm_repeats(cuda, n, p):
+    """One launch, and several: the same tensors give the same float64 sum, through every entry point that takes it."""
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    grads = [torch.randn(n, generator=gen, device=cuda), torch.randn(n // 3, generator=gen, device=cuda).half()[1:],
+             torch.randn(7, generator=gen, device=cuda, dtype=torch.float64)]
+    first = G.grad_norm(grads, p)
+    assert first.dtype == torch.float64
+    outs = [torch.empty_like(g) for g in grads]
+    for _ in range(5):
+        assert torch.equal(G.grad_norm(grads, p), first)
+        assert torch.equal(G.clip_grads(grads, 0.1, p, out=outs)[1], first)
+
+
+def test_limits_and_norms_at_the_ends_of_the_range(cuda):
+    g = torch.tensor([1.0, math.inf, -2.0], device=cuda)
+    outs, total = G.clip_grads([g], math.inf)
+    assert float(total) == math.inf and bool(outs[0].isnan().all())  # inf / inf, as torch's clipping
+    other = torch.nn.Parameter(torch.zeros(3, device=cuda))
+    other.grad = g.clone()
+    torch.nn.utils.clip_grad_norm_(other, math.inf)
+    assert torch.equal(other.grad.isnan(), outs[0].isnan())
+    tiny = torch.full((4,), 1e-170, device=cuda, dtype=torch.float64)
+    assert float(G.grad_norm([tiny])) == 0.0 and float(G.grad_norm([tiny], 1.0)) > 0.0
+    assert float(G.grad_norm([tiny * 1e15])) == pytest.approx(2e-155, rel=1e-12)
