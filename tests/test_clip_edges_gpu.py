@@ -9,6 +9,7 @@ import torch
 
 from gs_b200 import adam as A
 from gs_b200 import grad as G
+from gs_b200 import gs3d
 
 pytestmark = pytest.mark.gpu
 
@@ -253,3 +254,61 @@ def test_limits_and_norms_at_the_ends_of_the_range(cuda):
     tiny = torch.full((4,), 1e-170, device=cuda, dtype=torch.float64)
     assert float(G.grad_norm([tiny])) == 0.0 and float(G.grad_norm([tiny], 1.0)) > 0.0
     assert float(G.grad_norm([tiny * 1e15])) == pytest.approx(2e-155, rel=1e-12)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("n", [3, 4096, 30_011])
+def test_clipped_lean_step_by_every_norm(cuda, n, p, masked):
+    """The clipped lean step has the bits of clipping and then stepping, whichever norm and mask choose its kernel."""
+    vis = None
+    if masked:
+        vis = (torch.rand(n, device=cuda, generator=torch.Generator(device=cuda).manual_seed(n)) < 0.4).int()
+        vis[0] = 3
+    a = adam_state(n, cuda, n, lowp=(2, 5))
+    b = copies(a)
+    total = A.adam_step_lean(a, 12, vis, max_grad_norm=0.05, norm_type=p)
+    grads, want = G.clip_grads([x[1] for x in b], 0.05, p)
+    A.adam_step_lean([(x[0], g, *x[2:]) for x, g in zip(b, grads)], 12, vis)
+    flat = torch.cat([x[1].double().reshape(-1) for x in a])
+    exact = float(flat.abs().max() if p == math.inf else (flat.abs() ** p).sum() ** (1 / p))
+    # a float64 sum of fewer than 2^13 additions a path, rounded once to float32
+    assert abs(float(total) - exact) <= 2.0 ** -24 * 1.001 * exact and torch.equal(total, want)
+    for x, y in zip(a, b):
+        assert all(torch.equal(x[i], y[i]) for i in (0, 2, 3))
+    if masked:
+        start = adam_state(n, cuda, n, lowp=(2, 5))
+        assert all(torch.equal(x[i][vis == 0], y[i][vis == 0]) for x, y in zip(a, start) for i in (0, 2, 3))
+
+
+@pytest.mark.parametrize("stale", [False, True])
+@pytest.mark.parametrize("p", [2.0, math.inf])
+def test_sparse_optimizer_in_several_launches(cuda, monkeypatch, p, stale):
+    """More groups than a launch takes, or groups that a stale mask sends to the dense update: one norm over all of
+    them, then masked steps by that norm."""
+    n = 2003
+    vis = (torch.rand(n, device=cuda) < 0.4).int()
+    monkeypatch.setattr(gs3d._Rasterize, "track_visibility", False)  # as it was, when the optimizers have set it
+    monkeypatch.setattr(gs3d._Rasterize, "last_visibility", vis, raising=False)
+    shapes = [(n, *s) for s in (SHAPES_3DGS * 2)[:4 if stale else 11]] + ([(n + 1, 3)] if stale else [])
+    start = [torch.randn(s, device=cuda) for s in shapes]
+    a, b = ([t.clone().requires_grad_() for t in start] for _ in range(2))
+    kw = {"lr": 1e-3, "eps": 1e-15, "sparse": True, "lowp_moment_groups": ("g1", "g3")}
+    oa = A.FusedAdam([{"params": [t], "name": f"g{k}"} for k, t in enumerate(a)], max_grad_norm=0.3, grad_norm_type=p,
+                     **kw)
+    ob = A.FusedAdam([{"params": [t], "name": f"g{k}"} for k, t in enumerate(b)], **kw)
+    for _ in range(3):
+        for x, y in zip(a, b):
+            x.grad = torch.randn_like(x)
+            y.grad = x.grad.clone()
+        oa.step()
+        want = G.clip_grad_norm_(b, 0.3, p)
+        ob.step()
+        assert torch.equal(oa.grad_norm, want) and float(want) > 0.3
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+            assert all(torch.equal(oa.state[x][k], ob.state[y][k]) for k in ("exp_avg", "exp_avg_sq"))
+    assert oa.n_dense_fallbacks == (3 if stale else 0)
+    for x, t in zip(a, start):
+        if x.shape[0] == n:
+            assert torch.equal(x[vis == 0], t[vis == 0]) and not torch.equal(x, t)
