@@ -21,6 +21,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200) and the built libsplat_b200.so")
 
 
+def pytest_collection_modifyitems(items):
+    """The comparison with the reference's blend backward needs that kernel, which oracle/build.py builds where the
+    reference tree exists; without it those tests are skipped, as the other comparisons with the reference's kernels."""
+    from oracle.fastergs_ref import REF_LIB
+
+    if REF_LIB.exists():
+        return
+    skip = pytest.mark.skip(reason="the reference's blend backward is not built (oracle/build.py builds it where the "
+                                   "reference tree exists)")
+    for item in items:
+        if item.path.name == "test_gs3d_ref_backward_gpu.py":
+            item.add_marker(skip)
+
+
 def golden(name: str) -> dict:
     with np.load(GOLDEN / f"{name}.npz") as f:
         return {k: f[k] for k in f.files}
