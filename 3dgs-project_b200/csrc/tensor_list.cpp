@@ -209,7 +209,7 @@ PyObject* written(PyObject*, PyObject* seq) {
     for (Py_ssize_t i = 0; i < e.count; ++i) {
         const Entries group(e.items[i]);
         if (group.count == 0) bump(e.items[i]);
-        for (Py_ssize_t k = 0; k < group.count; ++k)
+        for (Py_ssize_t k = 0; k < group.count && k < 4; ++k)
             if (k != 1) bump(group.items[k]);
     }
     Py_RETURN_NONE;
