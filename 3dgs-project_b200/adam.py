@@ -163,7 +163,6 @@ class FusedAdam(torch.optim.Adam):
         by_key: dict[tuple, list] = {}
         grads: list[torch.Tensor] = []  # in the parameters' order, which the clip's sums follow
         masks: dict[tuple, torch.Tensor | None] = {}
-        counters: list[torch.Tensor] = []
         updated: list[torch.Tensor] = []
         for group in self.param_groups:
             if len(group["params"]) != 1:
@@ -183,7 +182,6 @@ class FusedAdam(torch.optim.Adam):
                 # densification concatenates float32 zeros to the moments, which promotes them; convert back
                 state["exp_avg"] = state["exp_avg"].to(moment_dtype)
                 state["exp_avg_sq"] = state["exp_avg_sq"].to(moment_dtype)
-            counters.append(state["step"])
             updated += param, state["exp_avg"], state["exp_avg_sq"]
             grad = param.grad if param.grad.is_contiguous() else param.grad.contiguous()
             step = int(state["step"].item()) + 1
@@ -202,17 +200,19 @@ class FusedAdam(torch.optim.Adam):
                                    state["exp_avg_sq"].data_ptr(), param.numel(), float(group["lr"]),
                                    param.numel() // max(param.shape[0], 1), int(lowp))
             entry._keep = grad
+            entry._counter = state["step"]
             grads.append(grad)
             by_key.setdefault(key, []).append(entry)
         clip = None
         if self.max_grad_norm is not None:
             clip = self._clip(grads, len(by_key) == 1 and len(grads) <= MAX_GROUPS)
-        for counter in counters:  # once all memory is had: a step that runs out of it has not happened
-            counter += 1
         for key, groups in by_key.items():
             kind, step, b1, b2, eps, dev = key[:6]
             for s in range(0, len(groups), MAX_GROUPS):
-                _launch(kind == "lean", groups[s:s + MAX_GROUPS], step, (b1, b2), eps, masks.get(key), dev, clip)
+                chunk = groups[s:s + MAX_GROUPS]
+                _launch(kind == "lean", chunk, step, (b1, b2), eps, masks.get(key), dev, clip)
+                for entry in chunk:  # a step that ran out of memory, or was refused, has not happened
+                    entry._counter += 1
         if clip is not None:
             gs_grad.written(updated)
 

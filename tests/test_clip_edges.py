@@ -99,6 +99,24 @@ def test_a_step_that_runs_out_of_memory_is_not_counted(monkeypatch, steps, count
         assert [s[0] for s in steps] == [n] * len(steps) and sum(s[1] for s in steps) == count
 
 
+@pytest.mark.parametrize("clip", [{}, {"max_grad_norm": 1.0}])
+def test_a_launch_that_is_refused_is_not_counted(monkeypatch, steps, clip):
+    params = [torch.nn.Parameter(torch.ones(3)) for _ in range(A.MAX_GROUPS + 3)]
+    for p in params:
+        p.grad = torch.ones(3)
+    opt = A.FusedAdam([{"params": [p]} for p in params], lr=1e-3, eps=1e-15, **clip)
+    monkeypatch.setattr(G, "grad_norm", lambda *args: torch.zeros(()))
+
+    def second_fails(lean, groups, *args):
+        if len(groups) < A.MAX_GROUPS:
+            raise RuntimeError("refused")
+
+    monkeypatch.setattr(A, "_launch", second_fails)
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    assert [float(opt.state[p]["step"]) for p in params] == [1.0] * A.MAX_GROUPS + [0.0] * 3
+
+
 def test_a_limit_set_between_steps_is_checked():
     opt = A.FusedAdam([torch.nn.Parameter(torch.zeros(3))], lr=1e-3, eps=1e-15, max_grad_norm=1.0)
     for bad in (-1.0, float("nan")):
