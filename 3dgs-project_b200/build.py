@@ -62,7 +62,7 @@ def build_tensors(force: bool = False, verbose: bool = False) -> Path | None:
         return None
     torch_dir = Path(torch.submodule_search_locations[0])
     src = CSRC / "tensor_list.cpp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", str(src), f"-I{torch_dir / 'include'}",
+    cmd = ["g++", "-O3", "-std=c++17", "-fPIC", "-shared", str(src), f"-I{torch_dir / 'include'}",
            f"-I{torch_dir / 'include/torch/csrc/api/include'}", f"-I{python_header().parent}",
            f"-I{Path(nvcc()).resolve().parent.parent / 'include'}", f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch_python"]

@@ -352,25 +352,26 @@ inline int size_of(int dtype) { return dtype == SPLAT_F32 ? 4 : dtype == SPLAT_F
 // A buffer of float32 or float64 values that is there.
 inline bool aligned(const void* p, bool f64) { return p && reinterpret_cast<uintptr_t>(p) % (f64 ? 8 : 4) == 0; }
 
-// A buffer of a call.
+// A buffer of a call: its first byte's address, doubled, with whether the call writes it in the lowest bit (addresses
+// have fewer than 63 bits), and the address behind its last byte.
 struct Range {
-    uintptr_t begin, end;
-    bool written;
+    uint64_t begin, end;
 };
 
 inline Range range_of(const void* p, unsigned long long bytes, bool written) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-    return {at, at + bytes, written};
+    const uint64_t at = reinterpret_cast<uintptr_t>(p);
+    return {at << 1 | (written ? 1u : 0u), at + bytes};
 }
 
 // No range that is written overlaps another one. Sorts them.
 inline bool apart(Range* s, int count) {
     std::sort(s, s + count, [](const Range& a, const Range& b) { return a.begin < b.begin; });
-    uintptr_t written_to = 0, read_to = 0;
+    uint64_t to[2] = {0, 0};  // where the ranges so far end that are read, that are written
     for (int i = 0; i < count; ++i) {
-        if (s[i].begin < written_to || (s[i].written && s[i].begin < read_to)) return false;
-        uintptr_t& to = s[i].written ? written_to : read_to;
-        to = std::max(to, s[i].end);
+        const uint64_t begin = s[i].begin >> 1;
+        const bool written = s[i].begin & 1;
+        if (begin < to[1] || (written && begin < to[0])) return false;
+        to[written] = std::max(to[written], s[i].end);
     }
     return true;
 }
