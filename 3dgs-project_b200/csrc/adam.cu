@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kThreads) k_adam(Table t) {
 }
 
 // The clipped step: k_adam with the factor, after the norm's kernels. It and they are bound by HBM: 3M Gaussians move
-// 4.96 GB in the step and 0.71 GB in the norm's pass, less the 64 MiB that this pass keeps in the L2 for the tiles taken
-// first here, and take 843 us (105 of them the norm's), 5.6 GB at 6.6 TB/s. A resident grid whose blocks loop over
+// 4.96 GB in the step and 0.71 GB in the norm's pass, less the 64 MiB that this pass leaves in the L2 for the tiles taken
+// first here, and take 846 us (105 of them the norm's), 5.6 GB at 6.6 TB/s. A resident grid whose blocks loop over
 // tiles took 935 us: blocks in step with one another load and store in turn.
 __global__ void __launch_bounds__(kThreads, 5)
     k_adam_clipped(const __grid_constant__ Table t, const __grid_constant__ gradnorm::Clip c) {
@@ -314,7 +314,10 @@ constexpr int kLeanList = 32 * kLeanIters;  // groups of four elements that a wa
 // any is used) and then deals them to its lanes in order: the update is dozens of instructions an element, which the
 // lanes of groups without one would sit through. Measured on 3M Gaussians with bfloat16 SH moments, against each thread
 // updating its own groups: 51% visible at random 574 us (611), visible in long runs 404 (405), without a mask, where
-// nothing is collected, 590 (615). Not unrolled: two groups in flight a thread took 638 us at random.
+// nothing is collected, 590 (615). On 1M: 10% visible at random 108 (130), 90% 221 (219), all 224 (224); the collecting
+// costs up to 0.4 us where it saves nothing, which shows below 256 Gaussians (2.3 us against 2.0 for four). Lanes that
+// keep their own groups where dealing saves no round took 220 at 90% and 1% longer everywhere else. Not unrolled: two
+// groups in flight a thread took 638 us at random on 3M.
 template <bool kLowp, bool kClip, bool kMasked, int kIters>
 __device__ __forceinline__ void lean_block(const LeanGroup& G, const LeanTable& t, long long base, int thread,
                                            uint16_t* list, float f) {
@@ -390,8 +393,8 @@ __global__ void __launch_bounds__(kThreads) k_adam_lean(const __grid_constant__ 
 // As k_adam_clipped. 1M Gaussians of which 35% are visible, at random: 171 us after the norm's 35, 753 MB from and to
 // HBM, more than the visible elements' 370 MB because rows of 12 to 180 bytes share their 32-byte sectors. 62% of the
 // issue slots are busy beside 4.5 TB/s, and loads ahead of the update made it slower.
-// With the mask six blocks an SM are faster than five (206 us against 219, the norm included), without it slower (3M
-// Gaussians in float32 773 us against 733).
+// With the mask six blocks an SM are faster than five (206 us against 219, the norm included in both), without it slower
+// (3M Gaussians in float32: this kernel alone 773 us against 733).
 template <bool kMasked>
 __global__ void __launch_bounds__(kThreads, kMasked ? 6 : 1)
     k_adam_lean_clipped(const __grid_constant__ LeanTable t, const __grid_constant__ gradnorm::Clip c) {

@@ -6,13 +6,14 @@
 // chunks of 16 KiB from the 16-byte boundary at or before their first element, so that all but the first and the last
 // 16 bytes of a tensor move as 16-byte vectors wherever it starts.
 //
-// The norm reads everything once and is bound by HBM: 103 us for the 708 MB of 3M Gaussians' gradients (6.9 TB/s, 1.05
-// of the measured copy rate; with lines that leave the L2 first, as a call that reads on wants them, 105). Squares are added in float64, which keeps float32's whole range (a square of 1e-25 or
-// 1e25 leaves it) and every bit of the result; it costs a conversion and a float64 multiply-add an element, hidden
-// behind the loads at 32 registers and all 64 warps of an SM (46 registers, for looking the next chunk up while this
-// one loads, cost 1% on 3M Gaussians and 13% on a ragged 16-bit list). Teams take every teams-th chunk: neighbouring
-// chunks a team, with one search for the tensor, took 109 us. A list of 300 16-bit tensors (91 MB) takes 22 us, with
-// 64% of the issue slots busy: the 32 elements that a thread adds of a chunk carry the search and the chunk's geometry.
+// The norm reads everything once and is bound by HBM: 102 us for the 708 MB of 3M Gaussians' gradients (6.9 TB/s, 1.06
+// of the measured copy rate; with lines that leave the L2 first, as a call that reads on wants them, 105). Squares are
+// added in float64, which keeps float32's whole range (a square of 1e-25 or 1e25 leaves it) and every bit of the result;
+// it costs a conversion and a float64 multiply-add an element, hidden behind the loads at 32 registers and all 64 warps
+// of an SM (46 registers, for looking the next chunk up while this one loads, cost 1% on 3M Gaussians and 13% on a ragged
+// 16-bit list). Teams take every teams-th chunk: neighbouring chunks a team, with one search for the tensor, took 109 us.
+// A list of 300 16-bit tensors (91 MB) takes 23 us, with 64% of the issue slots busy: the 32 elements that a thread adds
+// of a chunk carry the search and the chunk's geometry, and a conversion each. Which of these costs what is not known.
 //
 // Clipping reads the gradients again, since the factor needs all of them: 1M Gaussians (236 MB) clipped into other
 // buffers move 3 x 236 MB less the 64 MiB that the norm's pass leaves in the L2 and take 111.3 us (644 MB in 98 us would
@@ -35,14 +36,15 @@ constexpr int kNormBlocks = 4;  // per SM: all its threads
 constexpr uint32_t kKeepChunks = 4096;
 // Lists of up to 2048 chunks (32 MiB) leave the partials to the blocks that scale or step, each of which reduces them
 // for itself: one launch less, 3 us of the host's time, and on the device 6.5 against 7.4 us for clipping 20 thousand
-// 3D Gaussians' gradients and 31.9 against 32.6 for the step of 100 thousand. Longer lists have too many blocks for
-// that: the lean step of 1M Gaussians takes 214 us so and 207 after k_norm_finish.
+// 3D Gaussians' gradients and 31.9 against 32.6 for the step of 100 thousand (1444 chunks). Longer lists have too many
+// blocks for that: the lean step of 1M Gaussians (14408 chunks) takes 214 us so and 207 after k_norm_finish. Between
+// these two lengths nothing was measured.
 constexpr long long kDirectChunks = 2048;
 constexpr int kScaleThreads = kTeam;
 // Out of place a block scales one chunk: a resident grid that loops took 84 us where this takes 72 (1M Gaussians, 236 MB
 // read and written). In place most calls find a factor of 1 and end there, and blocks that only end cost time too: with
-// 8 chunks a block the call over 3M Gaussians takes 108.5 us when nothing changes and the scaling 225 us when something
-// does; with 1 it is 127.9 when nothing changes, with 32 the scaling takes 235.
+// 8 chunks a block the call over 3M Gaussians takes 105 us when nothing changes and 343 when something does; with 1 it
+// was 19 us slower when nothing changes, with 32 the scaling took 235 us instead of 225.
 constexpr unsigned int kScaleChunksInPlace = 8;
 constexpr unsigned int kScaleBlocks = 8;  // per SM, that a short list is spread over all the same
 

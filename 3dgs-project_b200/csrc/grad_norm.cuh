@@ -34,7 +34,8 @@ constexpr int kMaxPartials = 1024;  // of one launch
 // through distributed shared memory. Eight SMs are slower than all of them on the longer of these lists, but each launch
 // saved is 3 us of the host's time. The norm of 43 chunks (3000 3D Gaussians): 5.0 us on the device and 9.8 us a call,
 // against 3.5 and 12.7 in two launches. At 86 chunks clipping takes 12.3 us on the device and 16.0 a call, against 5.6
-// and 15.7 in two: there the device has caught up with the host.
+// and 15.7 in two: there the device has caught up with the host. In a captured graph, where the host's time does not
+// count, the longer of these lists would be faster in two launches too; the rule does not look at captures.
 constexpr int kSmallCluster = 8;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallChunks = 64;

@@ -8,11 +8,11 @@ The Adam steps of gs_b200.adam take max_grad_norm and clip as they read the grad
 
 Tensors are float32, bfloat16, float16 or float64 CUDA tensors, mixed in one call, each dense in its own order of
 dimensions (contiguous, transposed, channels-last), of any length and at any address. Sums are taken in float64 in an
-order that follows from the list's lengths and types, the addresses modulo 16 bytes and the device, so a call on the same
-tensors repeats bit for bit; copies at other addresses may differ in the last bits of the float64 sum. None of the calls
-waits for the device (error_if_nonfinite apart), and all can be captured into a CUDA graph. Nothing is recorded for
-autograd, except that tensors were written: as after torch's own in-place operations, a backward that needs their old
-values raises.
+order that follows from the list's lengths and types, the addresses modulo 16 bytes and the device, so a call on the
+same tensors repeats bit for bit; copies at other addresses may differ in the last bits of the float64 sum. None of the
+calls waits for the device (error_if_nonfinite apart), and all can be captured into a CUDA graph. Nothing is recorded
+for autograd, except that tensors were written: as after torch's own in-place operations, a backward that needs their
+old values raises.
 """
 from __future__ import annotations
 
@@ -171,8 +171,9 @@ def _check_finite(norm: torch.Tensor, norm_type) -> None:
 def grad_norm(grads, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """The norm of all elements of the tensors as one vector: 0-d, float32 (float64 when one of them is float64), on
     their device. norm_type: 1, 2 or inf. NaN when an element is NaN. Squares of float64 elements leave float64's range
-    beyond 1e154 (the norm is infinite) and below 1e-162 (they count as 0); those of the other types do not. No tensors: 0 on the CPU, as torch's clipping
-    gives. error_if_nonfinite raises for an infinite or NaN norm (which waits for the device)."""
+    beyond 1e154 (the norm is infinite) and below 1e-162 (they count as 0); those of the other types do not. No tensors:
+    0 on the CPU, as torch's clipping gives. error_if_nonfinite raises for an infinite or NaN norm (which waits for the
+    device)."""
     norm = norm_code(norm_type)
     tensors = _listed(grads)
     if not tensors:
