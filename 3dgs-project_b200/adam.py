@@ -163,7 +163,6 @@ class FusedAdam(torch.optim.Adam):
         by_key: dict[tuple, list] = {}
         grads: list[torch.Tensor] = []  # in the parameters' order, which the clip's sums follow
         masks: dict[tuple, torch.Tensor | None] = {}
-        updated: list[torch.Tensor] = []
         for group in self.param_groups:
             if len(group["params"]) != 1:
                 raise RuntimeError("more than one tensor in group")
@@ -182,7 +181,6 @@ class FusedAdam(torch.optim.Adam):
                 # densification concatenates float32 zeros to the moments, which promotes them; convert back
                 state["exp_avg"] = state["exp_avg"].to(moment_dtype)
                 state["exp_avg_sq"] = state["exp_avg_sq"].to(moment_dtype)
-            updated += param, state["exp_avg"], state["exp_avg_sq"]
             grad = param.grad if param.grad.is_contiguous() else param.grad.contiguous()
             step = int(state["step"].item()) + 1
             if not self.lean:
@@ -199,8 +197,8 @@ class FusedAdam(torch.optim.Adam):
                 entry = _LeanGroup(param.data_ptr(), grad.data_ptr(), state["exp_avg"].data_ptr(),
                                    state["exp_avg_sq"].data_ptr(), param.numel(), float(group["lr"]),
                                    param.numel() // max(param.shape[0], 1), int(lowp))
-            entry._keep = grad
             entry._counter = state["step"]
+            entry._updated = (param, grad, state["exp_avg"], state["exp_avg_sq"])
             grads.append(grad)
             by_key.setdefault(key, []).append(entry)
         clip = None
@@ -213,8 +211,8 @@ class FusedAdam(torch.optim.Adam):
                 _launch(kind == "lean", chunk, step, (b1, b2), eps, masks.get(key), dev, clip)
                 for entry in chunk:  # a step that ran out of memory, or was refused, has not happened
                     entry._counter += 1
-        if clip is not None:
-            gs_grad.written(updated)
+                if clip is not None:
+                    gs_grad.written([entry._updated for entry in chunk])
 
     def _check_clipped(self) -> None:
         """The clipped step's limit, which a caller may set anew between steps, and gradients: one norm is taken over

@@ -274,7 +274,8 @@ int check_list(const char* what, int count, const void* const* grads, const long
     for (int i = 0; i < count; ++i) {
         SPLAT_REQUIRE(n[i] >= 0, "%s: tensor %d has negative size", what, i);
         SPLAT_REQUIRE(dtypes[i] <= SPLAT_F64, "%s: tensor %d has an unknown type", what, i);
-        SPLAT_REQUIRE(n[i] <= (1ll << 45) / size_of(dtypes[i]), "%s: tensor %d has %lld elements", what, i, n[i]);  // 32 TiB
+        // 32 TiB
+        SPLAT_REQUIRE(n[i] <= (1ll << 45) / size_of(dtypes[i]), "%s: tensor %d has %lld elements", what, i, n[i]);
         SPLAT_REQUIRE(dtypes[i] != SPLAT_F64 || norm_f64, "%s: tensor %d is float64, the norm is not", what, i);
         if (n[i] == 0) continue;
         SPLAT_REQUIRE(grads[i], "%s: tensor %d has a null buffer", what, i);

@@ -419,7 +419,7 @@ int splat_grad_clip(int count, const void* const* grads, void* const* outs, cons
                     void* workspace, size_t workspace_bytes, void* stream);
 /* adam_step_multi / adam_step_multi_lean of the gradients grad * f, f from the norm over the groups of this call (with
  * SPLAT_NORM_GIVEN: from *norm). The gradients are left as they are. Parameters, moments and the norm overlap
- * neither one another nor a gradient (two groups may share one gradient). Bit-identical to splat_grad_clip followed by the
+ * neither one another nor a gradient (two groups may share one gradient). Bit-identical to splat_grad_clip and then the
  * step. The norm counts every gradient, those of primitives that the lean step's mask leaves out too. */
 int adam_step_multi_clipped(int count, const adam_group* groups, int step, double beta1, double beta2, double eps,
                             int norm_type, double max_norm, float* norm, void* workspace, size_t workspace_bytes,

@@ -112,8 +112,11 @@ def test_a_launch_that_is_refused_is_not_counted(monkeypatch, steps, clip):
             raise RuntimeError("refused")
 
     monkeypatch.setattr(A, "_launch", second_fails)
+    before = [p._version for p in params]
     with pytest.raises(RuntimeError, match="refused"):
         opt.step()
+    written = [p._version - v for p, v in zip(params, before)]  # what was launched has been written all the same
+    assert written == [1 if clip else 0] * A.MAX_GROUPS + [0] * 3
     assert [float(opt.state[p]["step"]) for p in params] == [1.0] * A.MAX_GROUPS + [0.0] * 3
 
 
